@@ -123,9 +123,9 @@ __device__ __forceinline__ float gelu_erf_f(float x) {
 }
 // The same GELU where the result is rounded to bf16 right away (the fused GeGLU epilogue of the bf16 GEMM): erf(x / sqrt 2)
 // = x Q(x^2) on |x| <= 4.4 (clamped: 1 - erf(4.4 / sqrt 2) = 1.1e-5), Q of degree 8 fitted to a maximum error of 3.4e-5 in
-// erf = 7.4e-5 in the GELU at worst (x ~ 4), 1/50 of a bf16 rounding step there.  No v_rcp / v_exp (7.7 cycles each) and the
-// Horner chain packs two values per v_pk_fma_f32: the epilogue's math is what a GeGLU tile waits for after its K loop.
-// Two values at a time, so that every step is a packed instruction (v_pk_mul_f32 / v_pk_fma_f32).
+// erf = 7.4e-5 in the GELU at worst (x ~ 4), 1/50 of a bf16 rounding step there.  No v_rcp / v_exp (7.7 cycles each): the
+// epilogue's math is what a GeGLU tile waits for after its K loop.  Two values at a time; the build keeps the packed f32
+// instructions off (Makefile), so each step is two scalar ones.
 typedef __attribute__((ext_vector_type(2))) float gelu_f32x2_t;
 __device__ __forceinline__ gelu_f32x2_t gelu_erf_bf16out_f2(gelu_f32x2_t x) {
   typedef gelu_f32x2_t v2;
