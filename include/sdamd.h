@@ -24,6 +24,8 @@ extern "C" {
 
 #define SDAMD_F32 0
 #define SDAMD_BF16 1
+#define SDAMD_E4M3 2 /* 8-bit blocks, see below */
+#define SDAMD_E5M2 3
 #define SDAMD_ACT_NONE 0
 #define SDAMD_ACT_QUICK_GELU 1 /* x*sigmoid(1.702x), clip.py:67 */
 #define SDAMD_ACT_SILU 2       /* diffusion.py:163 */
@@ -241,6 +243,53 @@ int sdamd_attention(const void* q, const void* k, const void* v, void* out, int 
                     int Skv, int d, long long q_bs, int q_rs, long long k_bs, int k_rs,
                     long long v_bs, int v_rs, long long o_bs, int o_rs, int causal, int dtype,
                     void* stream);
+
+/* ---- 8-bit blocks, and training of the transformer blocks (diffusion.py:109-137; no counterpart in the reference, which
+ * infers only).  Format: rows of K values are kept as KB = ceil(K / 128) blocks of 128 bytes, q [rows][KB*128] e4m3 / e5m2
+ * (OCP; zero bytes past K, 16-byte aligned), with one scale byte e per block standing for 2^(e-127): scale [rows][SP], SP =
+ * KB up to a multiple of 4 (4-byte aligned).  Weights (e4m3) share a byte over 128 rows: scale [ceil(N/128)][SP].
+ * A scale is the smallest power of two with max |finite x| <= max(type) * scale (1 for a block of zeros); values are rounded
+ * to nearest even.  NaN stays NaN; an infinity becomes NaN in e4m3 and stays in e5m2.
+ * fmt: SDAMD_E4M3 | SDAMD_E5M2.  Odd widths and element-aligned pointers are taken everywhere else. */
+/* x [rows] of K values, row stride ldx elements */
+int sdamd_quant8(const void* x, void* q, unsigned char* scale, long long rows, int K, long long ldx, int dtype, int fmt,
+                 void* stream);
+/* w[n * stride_n + k * stride_k] -> e4m3 in 128 x 128 blocks */
+int sdamd_quant8_weight(const void* w, void* q, unsigned char* scale, int N, int K, long long stride_n, long long stride_k,
+                        int dtype, void* stream);
+/* out [rows][K]; block_rows = 1 or 128 (weights) */
+int sdamd_dequant8(const void* q, const unsigned char* scale, void* out, long long rows, int K, int block_rows, int fmt,
+                   int out_dtype, void* stream);
+/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n] + residual[m][n]), dense; x: blocks of type fmt (x_dtype == fmt), or at
+ * most sdamd_linear8_raw_rows() dense rows of x_dtype F32 / BF16 that the kernel quantises to fmt itself; w: e4m3 weight
+ * blocks.  out and residual are out_dtype.  BF16: the scaled 8-bit matrix instruction (its internal sums are good to about
+ * 1e-5 of the result); F32: exact products summed in f32 at half the rate.  act: none, quick-gelu, silu. */
+int sdamd_linear8_raw_rows(void);
+int sdamd_linear8(const void* x, const unsigned char* x_scale, const void* w, const unsigned char* w_scale, void* out,
+                  const float* bias, const void* residual, int M, int N, int K, int act, int x_dtype, int fmt,
+                  int out_dtype, void* stream);
+/* dw[n][k] = sum_t dy[t][n] x8[t][k], db[n] = sum_t dy[t][n] (db may be null); dy [T][N] bf16, x8 row blocks of type fmt.
+ * Exact products, f32 sums in a fixed order.  ws >= sdamd_linear8_weight_grad_ws_bytes(T, N, K), which may be 0. */
+size_t sdamd_linear8_weight_grad_ws_bytes(int T, int N, int K);
+int sdamd_linear8_weight_grad(const void* dy, const void* x8, const unsigned char* x8_scale, float* dw, float* db, void* ws,
+                              size_t ws_bytes, int T, int N, int K, int fmt, void* stream);
+/* LayerNorm forward with its statistics mean, rstd [rows] f32; y: F32 / BF16 [rows][C], or row blocks with y_scale
+ * (out_dtype SDAMD_E4M3 / SDAMD_E5M2; y_scale null otherwise).  C <= 12288. */
+int sdamd_layernorm_train(const void* x, void* y, unsigned char* y_scale, const float* gamma, const float* beta, float* mean,
+                          float* rstd, int rows, int C, float eps, int dtype, int out_dtype, void* stream);
+/* its gradients: xh = (x - mean) rstd, a = dy gamma, dx = rstd (a - sum(a)/C - xh sum(a xh)/C) (+ residual, of dx_dtype),
+ * dgamma = sum_rows dy xh, dbeta = sum_rows dy (f32, fixed order).  x: F32 / BF16, or row blocks with x_scale. */
+size_t sdamd_layernorm_backward_ws_bytes(int rows, int C);
+int sdamd_layernorm_backward(const void* dy, const void* x, const unsigned char* x_scale, const float* gamma,
+                             const float* mean, const float* rstd, const void* residual, void* dx, float* dgamma,
+                             float* dbeta, void* ws, size_t ws_bytes, int rows, int C, int dy_dtype, int x_dtype,
+                             int dx_dtype, void* stream);
+/* h [rows][2F] (value | gate) -> out [rows][F] = value * gelu_erf(gate) and h's row blocks (fmt) */
+int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt,
+                      void* stream);
+/* dh [rows][2F] = (dout gelu(gate) | dout value gelu'(gate)); h: F32 / BF16, or row blocks with h_scale */
+int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, long long rows, int F,
+                         int dout_dtype, int h_dtype, int dh_dtype, void* stream);
 
 #ifdef __cplusplus
 }

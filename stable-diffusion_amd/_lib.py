@@ -55,6 +55,18 @@ SIGNATURES = {
     "sdamd_conv3x3_cin_small": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "sdamd_conv3x3_cout_small": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "sdamd_attention": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _ll, _i, _ll, _i, _ll, _i, _ll, _i, _i, _i, _vp]),
+    "sdamd_quant8": (_i, [_vp, _vp, _vp, _ll, _i, _ll, _i, _i, _vp]),
+    "sdamd_quant8_weight": (_i, [_vp, _vp, _vp, _i, _i, _ll, _ll, _i, _vp]),
+    "sdamd_dequant8": (_i, [_vp, _vp, _vp, _ll, _i, _i, _i, _i, _vp]),
+    "sdamd_linear8_raw_rows": (_i, []),
+    "sdamd_linear8": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "sdamd_linear8_weight_grad_ws_bytes": (_sz, [_i, _i, _i]),
+    "sdamd_linear8_weight_grad": (_i, [_vp] * 6 + [_sz] + [_i] * 4 + [_vp]),
+    "sdamd_layernorm_train": (_i, [_vp] * 7 + [_i, _i, _f, _i, _i, _vp]),
+    "sdamd_layernorm_backward_ws_bytes": (_sz, [_i, _i]),
+    "sdamd_layernorm_backward": (_i, [_vp] * 11 + [_sz] + [_i] * 5 + [_vp]),
+    "sdamd_geglu_train": (_i, [_vp] * 4 + [_ll, _i, _i, _i, _vp]),
+    "sdamd_geglu_backward": (_i, [_vp] * 4 + [_ll, _i, _i, _i, _i, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,286 @@
+// 8-bit blocks (blocks8.h): quantise, dequantise, and GeGLU (diffusion.py:128-130) with its pre-activation kept in them.
+// All of it is bound by HBM: one pass, 16-byte loads, nothing read twice.
+#include "blocks8.h"
+
+// ---- rows -> blocks.  q [rows][KB*128], scale [rows][SP]; 16 lanes hold a block, a workgroup takes 16 * UN blocks.
+template <typename T, int UN>
+__global__ __launch_bounds__(256) void quant8_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
+                                                     unsigned char* __restrict__ scale, unsigned nblk, int KB, int K,
+                                                     long long ldx, int SP, int fmt) {
+  const int sub = threadIdx.x & 15;
+  const unsigned b0 = blockIdx.x * (16u * UN) + (threadIdx.x >> 4);
+  Raw8<T> raw[UN];
+  unsigned row[UN], kb[UN];
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {     // every block's values are requested before the first is used
+    const unsigned b = min(b0 + 16u * u, nblk - 1);
+    row[u] = b / (unsigned)KB;
+    kb[u] = b - row[u] * (unsigned)KB;
+    const int c = (int)kb[u] * B8_BLOCK + sub * 8;
+    raw[u] = raw8_load(x + (long long)row[u] * ldx, c, K);
+  }
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    float v[8];
+    raw8_get(raw[u], (int)kb[u] * B8_BLOCK + sub * 8, K, v);
+    const int e = b8_exponent_of(b8_max16(b8_mag8(v)), fmt);
+    if (b0 + 16u * u < nblk) {
+      *reinterpret_cast<u32x2_t*>(q + ((size_t)row[u] * KB + kb[u]) * B8_BLOCK + sub * 8) = b8_pack8(v, e, fmt);
+      if (sub == 0) scale[(size_t)row[u] * SP + kb[u]] = (unsigned char)e;
+      if (kb[u] == (unsigned)KB - 1 && KB + sub < SP) scale[(size_t)row[u] * SP + KB + sub] = 127;
+    }
+  }
+}
+
+// ---- weights -> 128 x 128 blocks.  One workgroup per block; the weight has any strides (w and w.t() alike): lanes run
+// along the shorter stride, the bytes turn in LDS and leave in rows.
+template <typename T>
+__global__ __launch_bounds__(256) void quant8_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ q,
+                                                            unsigned char* __restrict__ scale, int N, int K, long long sn,
+                                                            long long sk, int KB, int SP) {
+  __shared__ __attribute__((aligned(16))) unsigned char tile[128 * 132];
+  __shared__ unsigned red[4];
+  const int n0 = blockIdx.y * B8_BLOCK, k0 = blockIdx.x * B8_BLOCK, t = threadIdx.x;
+  const bool along_n = sn < sk;
+  float v[64];
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    const int a = i * 2 + (t >> 7), b = t & 127;
+    const int n = n0 + (along_n ? b : a), k = k0 + (along_n ? a : b);
+    v[i] = n < N && k < K ? Cvt<T>::ld(w + n * sn + k * sk) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 64; ++i) m = max(m, b8_mag(v[i]));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+  if ((t & 63) == 0) red[t >> 6] = m;
+  __syncthreads();
+  const int e = b8_exponent<8>(max(max(red[0], red[1]), max(red[2], red[3])));
+  const float inv = b8_inverse(e);
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    const int a = i * 2 + (t >> 7), b = t & 127;
+    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[i] * inv, 0.f, 0, false);
+    tile[along_n ? b * 132 + a : a * 132 + b] = (unsigned char)c;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int d = i * 256 + t, r = d >> 5, c = (d & 31) * 4;
+    if (n0 + r < N)
+      *reinterpret_cast<unsigned*>(q + ((size_t)(n0 + r) * KB + blockIdx.x) * B8_BLOCK + c) = *reinterpret_cast<const unsigned*>(tile + r * 132 + c);
+  }
+  if (t == 0) scale[(size_t)blockIdx.y * SP + blockIdx.x] = (unsigned char)e;
+  if ((int)blockIdx.x == KB - 1 && KB + t < SP) scale[(size_t)blockIdx.y * SP + KB + t] = 127;
+}
+
+// ---- blocks -> the values they stand for
+template <typename TO>
+__global__ __launch_bounds__(256) void dequant8_kernel(const unsigned char* __restrict__ q, const unsigned char* __restrict__ scale,
+                                                       TO* __restrict__ out, unsigned nblk, int KB, int K, int SP, int row_shift, int fmt) {
+  const int sub = threadIdx.x & 15;
+  const unsigned b = blockIdx.x * 16u + (threadIdx.x >> 4);
+  if (b >= nblk) return;
+  const unsigned row = b / (unsigned)KB, kb = b - row * (unsigned)KB;
+  const int c = (int)kb * B8_BLOCK + sub * 8;
+  if (c >= K) return;
+  float v[8];
+  b8_unpack8(*reinterpret_cast<const u32x2_t*>(q + (size_t)b * B8_BLOCK + sub * 8), scale[(size_t)(row >> row_shift) * SP + kb], fmt, v);
+  row_store8(out + (size_t)row * K + c, K - c, v);
+}
+
+// ---- GeGLU that keeps its input in 8 bits: h [rows][2F] -> out [rows][F] = value * gelu(gate), and h's blocks.
+// F % 128 == 0: the 16 lanes that hold a value block hold the gate block of the same columns too, so h is read once.
+template <typename T>
+__global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned char* __restrict__ q,
+                                                          unsigned char* __restrict__ scale, unsigned nblk, int FB, int SP, int fmt) {
+  const int sub = threadIdx.x & 15;
+  const unsigned b = blockIdx.x * 16u + (threadIdx.x >> 4);
+  const unsigned bb = min(b, nblk - 1), row = bb / (unsigned)FB, fb = bb - row * (unsigned)FB;
+  const size_t vb = (size_t)row * 2 * FB + fb, gb = vb + FB;          // block numbers in h
+  float v[8], g[8], o[8];
+  const Raw8<T> rv = raw8_load(h + vb * B8_BLOCK, sub * 8, B8_BLOCK), rg = raw8_load(h + gb * B8_BLOCK, sub * 8, B8_BLOCK);
+  raw8_get(rv, sub * 8, B8_BLOCK, v);
+  raw8_get(rg, sub * 8, B8_BLOCK, g);
+  const int ev = b8_exponent_of(b8_max16(b8_mag8(v)), fmt), eg = b8_exponent_of(b8_max16(b8_mag8(g)), fmt);
+  if (b >= nblk) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
+  row_store8(out + (size_t)bb * B8_BLOCK + sub * 8, 8, o);
+  *reinterpret_cast<u32x2_t*>(q + vb * B8_BLOCK + sub * 8) = b8_pack8(v, ev, fmt);
+  *reinterpret_cast<u32x2_t*>(q + gb * B8_BLOCK + sub * 8) = b8_pack8(g, eg, fmt);
+  if (sub == 0) { scale[(size_t)row * SP + fb] = (unsigned char)ev; scale[(size_t)row * SP + FB + fb] = (unsigned char)eg; }
+  if (fb == (unsigned)FB - 1 && 2 * FB + sub < SP) scale[(size_t)row * SP + 2 * FB + sub] = 127;
+}
+// any F: a value's block and its gate's do not line up, so the blocks come from quant8_kernel and this pass gates
+template <typename T>
+__global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned nvec, int VR, int F) {
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= nvec) return;
+  const unsigned row = i / (unsigned)VR;
+  const int c = (int)(i - row * (unsigned)VR) * 8;
+  const T* hr = h + (size_t)row * 2 * F;
+  float v[8], g[8], o[8];
+  row_load8(hr, c, F, v);
+  row_load8(hr + F, c, F, g);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
+  row_store8(out + (size_t)row * F + c, F - c, o);
+}
+
+// gelu(x) = x Phi(x) and its slope Phi(x) + x phi(x), erf as in gelu_erf_f (its exponential is phi's)
+__device__ __forceinline__ void gelu_slope(float x, float& gelu, float& slope) {
+  const float z = __builtin_fabsf(x) * 0.70710678118654752440f;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
+  float poly = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  poly = __builtin_fmaf(poly, t, 1.421413741f);
+  poly = __builtin_fmaf(poly, t, -0.284496736f);
+  poly = __builtin_fmaf(poly, t, 0.254829592f);
+  const float e = __builtin_amdgcn_exp2f(-(z * z) * 1.4426950408889634f);
+  const float tail = 0.5f * poly * t * e;                              // Phi(-|x|)
+  const float cdf = x < 0.f ? tail : 1.0f - tail;
+  gelu = x * cdf;
+  slope = __builtin_fmaf(x * 0.39894228040143267794f, e, cdf);
+}
+
+// ---- GeGLU backward: dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
+// (TH = unsigned char)
+template <typename TD, typename TH, typename TO>
+__global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restrict__ dout, const TH* __restrict__ h,
+                                                             const unsigned char* __restrict__ scale, TO* __restrict__ dh,
+                                                             unsigned nvec, int VR, int F, int ldh, int SP, int fmt) {
+  const unsigned i = blockIdx.x * 256u + threadIdx.x;
+  if (i >= nvec) return;
+  const unsigned row = i / (unsigned)VR;
+  const int c = (int)(i - row * (unsigned)VR) * 8;
+  const TH* hr = h + (size_t)row * ldh;
+  float d[8], v[8], g[8], dv[8], dg[8];
+  row_load8(dout + (size_t)row * F, c, F, d);
+  if constexpr (sizeof(TH) == 1) {
+    const unsigned char* sr = scale + (size_t)row * SP;
+    if (F % 8 == 0) {
+      const u32x2_t qv = *reinterpret_cast<const u32x2_t*>(hr + c), qg = *reinterpret_cast<const u32x2_t*>(hr + F + c);
+      b8_unpack8(qv, sr[c / B8_BLOCK], fmt, v);
+      b8_unpack8(qg, sr[(F + c) / B8_BLOCK], fmt, g);
+    } else {                         // the gates start at any byte and may change block inside the vector
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int cc = min(c + j, F - 1);
+        float o[8];
+        b8_unpack8((u32x2_t){(unsigned)hr[cc], 0u}, sr[cc / B8_BLOCK], fmt, o); v[j] = o[0];
+        b8_unpack8((u32x2_t){(unsigned)hr[F + cc], 0u}, sr[(F + cc) / B8_BLOCK], fmt, o); g[j] = o[0];
+      }
+    }
+  } else {
+    row_load8(hr, c, F, v);
+    row_load8(hr + F, c, F, g);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float ge, sl;
+    gelu_slope(g[j], ge, sl);
+    dv[j] = d[j] * ge;
+    dg[j] = d[j] * v[j] * sl;
+  }
+  row_store8(dh + (size_t)row * 2 * F + c, F - c, dv);
+  row_store8(dh + (size_t)row * 2 * F + F + c, F - c, dg);
+}
+
+// ---------------------------------------------------------------------------------------------
+// host entry points
+// ---------------------------------------------------------------------------------------------
+static bool is_fmt(int f) { return f == SDAMD_E4M3 || f == SDAMD_E5M2; }
+static bool is_val(int d) { return d == SDAMD_F32 || d == SDAMD_BF16; }
+
+extern "C" int sdamd_quant8(const void* x, void* q, unsigned char* scale, long long rows, int K, long long ldx, int dtype, int fmt, void* stream) {
+  SD_CHECK(is_val(dtype) && is_fmt(fmt), "quant8: unsupported dtypes in=%d out=%d", dtype, fmt);
+  SD_CHECK(rows > 0 && K > 0 && K <= (1 << 30) && ldx >= 0, "quant8: bad shape rows=%lld K=%d", rows, K);
+  const int KB = b8_kblocks(K);
+  SD_CHECK(rows * (long long)KB < (1ll << 31), "quant8: too large, rows=%lld K=%d", rows, K);
+  const unsigned nblk = (unsigned)(rows * KB);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == SDAMD_BF16)
+    quant8_kernel<bf16_t, 2><<<(nblk + 31) / 32, 256, 0, st>>>((const bf16_t*)x, (unsigned char*)q, scale, nblk, KB, K, ldx, b8_scale_stride(K), fmt);
+  else
+    quant8_kernel<float, 2><<<(nblk + 31) / 32, 256, 0, st>>>((const float*)x, (unsigned char*)q, scale, nblk, KB, K, ldx, b8_scale_stride(K), fmt);
+  SD_LAUNCH_CHECK("quant8");
+  return 0;
+}
+
+extern "C" int sdamd_quant8_weight(const void* w, void* q, unsigned char* scale, int N, int K, long long sn, long long sk, int dtype, void* stream) {
+  SD_CHECK(is_val(dtype), "quant8_weight: unsupported dtype %d", dtype);
+  SD_CHECK(N > 0 && K > 0 && K <= (1 << 30) && sn >= 0 && sk >= 0, "quant8_weight: bad shape N=%d K=%d", N, K);
+  const int KB = b8_kblocks(K), NB = b8_kblocks(N);
+  SD_CHECK(NB <= 65535, "quant8_weight: N=%d is too large", N);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == SDAMD_BF16)
+    quant8_weight_kernel<bf16_t><<<dim3(KB, NB), 256, 0, st>>>((const bf16_t*)w, (unsigned char*)q, scale, N, K, sn, sk, KB, b8_scale_stride(K));
+  else
+    quant8_weight_kernel<float><<<dim3(KB, NB), 256, 0, st>>>((const float*)w, (unsigned char*)q, scale, N, K, sn, sk, KB, b8_scale_stride(K));
+  SD_LAUNCH_CHECK("quant8_weight");
+  return 0;
+}
+
+extern "C" int sdamd_dequant8(const void* q, const unsigned char* scale, void* out, long long rows, int K, int block_rows, int fmt, int out_dtype, void* stream) {
+  SD_CHECK(is_val(out_dtype) && is_fmt(fmt), "dequant8: unsupported dtypes in=%d out=%d", fmt, out_dtype);
+  SD_CHECK(rows > 0 && K > 0 && K <= (1 << 30) && (block_rows == 1 || block_rows == B8_BLOCK), "dequant8: bad shape rows=%lld K=%d block_rows=%d", rows, K, block_rows);
+  const int KB = b8_kblocks(K);
+  SD_CHECK(rows * (long long)KB < (1ll << 31), "dequant8: too large, rows=%lld K=%d", rows, K);
+  const unsigned nblk = (unsigned)(rows * KB);
+  const int shift = block_rows == 1 ? 0 : 7, SP = b8_scale_stride(K);
+  hipStream_t st = (hipStream_t)stream;
+  if (out_dtype == SDAMD_BF16)
+    dequant8_kernel<bf16_t><<<(nblk + 15) / 16, 256, 0, st>>>((const unsigned char*)q, scale, (bf16_t*)out, nblk, KB, K, SP, shift, fmt);
+  else
+    dequant8_kernel<float><<<(nblk + 15) / 16, 256, 0, st>>>((const unsigned char*)q, scale, (float*)out, nblk, KB, K, SP, shift, fmt);
+  SD_LAUNCH_CHECK("dequant8");
+  return 0;
+}
+
+template <typename T>
+static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned char* scale, long long rows, int F, int fmt, hipStream_t st) {
+  const int SP = b8_scale_stride(2 * F);
+  if (F % B8_BLOCK == 0) {
+    const unsigned nblk = (unsigned)(rows * (F / B8_BLOCK));
+    geglu_train_kernel<T><<<(nblk + 15) / 16, 256, 0, st>>>(h, out, q, scale, nblk, F / B8_BLOCK, SP, fmt);
+  } else {
+    const int KB = b8_kblocks(2 * F), VR = (F + 7) / 8;
+    const unsigned nblk = (unsigned)(rows * KB), nvec = (unsigned)(rows * VR);
+    quant8_kernel<T, 2><<<(nblk + 31) / 32, 256, 0, st>>>(h, q, scale, nblk, KB, 2 * F, 2 * F, SP, fmt);
+    geglu_rows_kernel<T><<<(nvec + 255) / 256, 256, 0, st>>>(h, out, nvec, VR, F);
+  }
+}
+
+extern "C" int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt, void* stream) {
+  SD_CHECK(is_val(dtype) && is_fmt(fmt), "geglu_train: unsupported dtypes h=%d kept=%d", dtype, fmt);
+  SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_train: bad shape rows=%lld F=%d", rows, F);
+  SD_CHECK(rows * (long long)((F + 7) / 8) < (1ll << 31), "geglu_train: too large, rows=%lld F=%d", rows, F);
+  if (dtype == SDAMD_BF16) geglu_train_launch<bf16_t>((const bf16_t*)h, (bf16_t*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
+  else geglu_train_launch<float>((const float*)h, (float*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
+  SD_LAUNCH_CHECK("geglu_train");
+  return 0;
+}
+
+extern "C" int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, long long rows, int F,
+                                    int dout_dtype, int h_dtype, int dh_dtype, void* stream) {
+  SD_CHECK(is_val(dout_dtype) && is_val(dh_dtype) && (is_val(h_dtype) || is_fmt(h_dtype)), "geglu_backward: unsupported dtypes dout=%d h=%d dh=%d",
+           dout_dtype, h_dtype, dh_dtype);
+  SD_CHECK(!is_fmt(h_dtype) || h_scale, "geglu_backward: 8-bit h without its scales");
+  SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_backward: bad shape rows=%lld F=%d", rows, F);
+  const int VR = (F + 7) / 8;
+  SD_CHECK(rows * (long long)VR < (1ll << 31), "geglu_backward: too large, rows=%lld F=%d", rows, F);
+  const unsigned nvec = (unsigned)(rows * VR);
+  hipStream_t st = (hipStream_t)stream;
+  const int SP = b8_scale_stride(2 * F), ldq = b8_kblocks(2 * F) * B8_BLOCK;
+#define GB_LAUNCH(TD, TH, TO, LD) \
+  geglu_backward_kernel<TD, TH, TO><<<(nvec + 255) / 256, 256, 0, st>>>((const TD*)dout, (const TH*)h, h_scale, (TO*)dh, nvec, VR, F, LD, SP, h_dtype)
+#define GB_H(TD, TO) \
+  { if (h_dtype == SDAMD_F32) GB_LAUNCH(TD, float, TO, 2 * F); else if (h_dtype == SDAMD_BF16) GB_LAUNCH(TD, bf16_t, TO, 2 * F); else GB_LAUNCH(TD, unsigned char, TO, ldq); }
+  if (dout_dtype == SDAMD_F32) { if (dh_dtype == SDAMD_F32) GB_H(float, float) else GB_H(float, bf16_t) }
+  else { if (dh_dtype == SDAMD_F32) GB_H(bf16_t, float) else GB_H(bf16_t, bf16_t) }
+#undef GB_H
+#undef GB_LAUNCH
+  SD_LAUNCH_CHECK("geglu_backward");
+  return 0;
+}

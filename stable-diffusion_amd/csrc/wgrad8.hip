@@ -1,0 +1,287 @@
+// Weight and bias gradient of a Linear from the 8-bit checkpoint of its input (blocks8.h):
+//   dW[n][k] = sum_t dy[t][n] x8[t][k],   db[n] = sum_t dy[t][n];   dy [T][N] bf16, x8 [T][KB*128] with a scale per row and 128
+// The reduction runs over tokens, along which the scales change, so the 8-bit instruction (one scale per operand row)
+// cannot take x8.  Its bytes go to bf16 on the way into LDS, scaled: bf16 holds every such value exactly, so all products
+// are exact and the sums are f32, whatever the checkpoint's type.  Bound by the bf16 matrix rate for wide layers.
+//
+// Workgroup tile BT_N x BT_K of dW, token steps of 64, two LDS buffers.  Both operands arrive as rows of one token and are
+// needed as columns of 8 tokens: ds_read_b64_tr_b16 turns 4 x 16 blocks on the way out of LDS.  A row's 32-byte units (16
+// columns) are permuted by f(t) = (t & 3) | ((t >> 3) & 1) << 2: the 16 rows such a read touches fall on all 64 banks.
+// "A" of the instruction = columns k, "B" = columns n: a lane ends up with 4 consecutive k of one n.
+// db costs one more instruction per n tile and step, against a row of ones, in the waves of the first k tile.
+// Few tiles and many tokens: the tokens are split over workgroups, which leave f32 partial sums; a second launch adds them
+// in a fixed order (no atomics: the same bits every run).
+#include "blocks8.h"
+#include "gemm_common.h"
+
+typedef __attribute__((address_space(3))) void lds_voidw_t;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2w_t;
+typedef f32x4_t __attribute__((aligned(4))) w8_f32x4_a4;
+
+static __device__ __attribute__((aligned(256))) const unsigned int g_wgrad_zero[4] = {0};
+
+struct W8Args {
+  const bf16_t* dy;
+  const unsigned char* q;
+  const unsigned char* qs;
+  float* dw;        // [splits][N][K] partial sums, or the result
+  float* db;        // [splits][N], or the result; null: not wanted
+  int T, N, K, KB, SP;
+  int tiles_n, tiles_k, steps;   // steps: token steps of 64 per split
+};
+
+template <int FMT> __device__ __forceinline__ void w8_to_bf16(u32x4_t v, float s, u32x4_t& lo, u32x4_t& hi) {
+  unsigned o[8];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    bf16x2w_t a, b;
+    if constexpr (FMT == SDAMD_E4M3) {
+      a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)v[h], s, false);
+      b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)v[h], s, true);
+    } else {
+      a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)v[h], s, false);
+      b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((int)v[h], s, true);
+    }
+    o[2 * h] = __builtin_bit_cast(unsigned, a);
+    o[2 * h + 1] = __builtin_bit_cast(unsigned, b);
+  }
+  lo = (u32x4_t){o[0], o[1], o[2], o[3]};
+  hi = (u32x4_t){o[4], o[5], o[6], o[7]};
+}
+__device__ __forceinline__ int w8_swz(int t) { return (t & 3) | (((t >> 3) & 1) << 2); }
+
+// DMA: rows of dy are 16-byte aligned (N % 8 == 0 and an aligned base) and go straight to LDS; otherwise through registers
+template <int BT_N, int BT_K, int WGN, int WGK, int FMT, bool DMA>
+__global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
+  constexpr int NT = 64 * WGN * WGK, TN = BT_N / WGN / 16, TK = BT_K / WGK / 16;
+  constexpr int ROWN = BT_N * 2, ROWK = BT_K * 2, STAGE = 64 * (ROWN + ROWK);
+  constexpr int QI = 64 * BT_K / 16 / NT;                  // 16-byte pieces of x8 per thread and step
+  constexpr int DI = 64 * ROWN / 16 / NT;                  // 16-byte pieces of dy per thread and step
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave % WGN, wk = wave / WGN, r16 = lane & 15, g = lane >> 4;
+
+  int id = blockIdx.x;                                     // neighbouring tiles on one XCD (see gemm8.hip)
+  {
+    const int total = p.tiles_n * p.tiles_k, per = total / 8, rem = total % 8, x = id % 8, r = id / 8;
+    id = x * per + min(x, rem) + r;
+  }
+  const int n0 = (id / p.tiles_k) * BT_N, k0 = (id % p.tiles_k) * BT_K;
+  const int t_begin = blockIdx.y * p.steps * 64, t_end = min(p.T, t_begin + p.steps * 64);
+  const int steps = (t_end - t_begin + 63) / 64;           // (the launcher leaves no split empty)
+
+  auto stage_dy_dma = [&](int s, int buf) {
+#pragma unroll
+    for (int i = 0; i < DI; ++i) {
+      const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
+      const int col = (((c >> 1) ^ w8_swz(t)) * 2 + (c & 1)) * 8;       // column whose 16 bytes belong at this place
+      const int tok = t_begin + s * 64 + t;
+      const void* src = tok < t_end && n0 + col < p.N ? (const void*)(p.dy + (size_t)tok * p.N + n0 + col) : (const void*)g_wgrad_zero;
+      const unsigned l = (unsigned)(unsigned long)(lds_voidw_t*)(smem + buf * STAGE + (i * NT + (tid & ~63)) * 16);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(src) : "memory", "m0");
+    }
+  };
+  Raw8<bf16_t> rd[DMA ? 1 : DI];
+  auto load_dy = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < DI; ++i) {
+      const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
+      rd[DMA ? 0 : i] = raw8_load(p.dy + (size_t)min(t_begin + s * 64 + t, p.T - 1) * p.N, n0 + c * 8, p.N);
+    }
+  };
+  auto write_dy = [&](int s, int buf) {
+#pragma unroll
+    for (int i = 0; i < DI; ++i) {
+      const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
+      float v[8];
+      raw8_get(rd[DMA ? 0 : i], n0 + c * 8, p.N, v);
+      u32x4_t o = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
+      if (t_begin + s * 64 + t >= t_end) o = (u32x4_t){0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4_t*>(smem + buf * STAGE + t * ROWN + (((c >> 1) ^ w8_swz(t)) * 2 + (c & 1)) * 16) = o;
+    }
+  };
+  u32x4_t rq[QI];
+  int rs[QI];
+  auto load_q = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+      const int piece = i * NT + tid, t = piece / (BT_K / 16), u = piece % (BT_K / 16);
+      const size_t tok = min(t_begin + s * 64 + t, p.T - 1);
+      const int kc = min(k0 + u * 16, p.KB * B8_BLOCK - 16);            // (columns past the row: some of it, never stored)
+      rq[i] = *reinterpret_cast<const u32x4_t*>(p.q + tok * p.KB * B8_BLOCK + kc);
+      rs[i] = p.qs[tok * p.SP + kc / B8_BLOCK];
+    }
+  };
+  auto write_q = [&](int s, int buf) {
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+      const int piece = i * NT + tid, t = piece / (BT_K / 16), u = piece % (BT_K / 16);
+      u32x4_t lo, hi;
+      w8_to_bf16<FMT>(rq[i], b8_scale(rs[i]), lo, hi);
+      if (t_begin + s * 64 + t >= t_end) { lo = (u32x4_t){0u, 0u, 0u, 0u}; hi = lo; }
+      char* d = smem + buf * STAGE + 64 * ROWN + t * ROWK + ((u ^ w8_swz(t)) << 5);
+      *reinterpret_cast<u32x4_t*>(d) = lo;
+      *reinterpret_cast<u32x4_t*>(d + 16) = hi;
+    }
+  };
+  // 8 tokens (8 g .. of a 32-token half) of the 16 columns of unit u
+  auto frag = [&](const char* base, int row_bytes, int half, int u) {
+    typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+    const int t = half * 32 + g * 8 + (r16 >> 2), f = w8_swz(t);        // (t and t + 4 have the same f)
+    const char* a = base + t * row_bytes + ((u ^ f) << 5) + (r16 & 3) * 8;
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)a);
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(a + 4 * row_bytes));
+    typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+    return __builtin_bit_cast(bf16x8_t, (s16x8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  };
+
+  f32x4_t acc[TK][TN], accb[TN];
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    accb[j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < TK; ++i) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  }
+  const bool want_db = p.db && k0 == 0 && wk == 0;
+  const __bf16 one = (__bf16)1.0f;
+  const bf16x8_t ones = {one, one, one, one, one, one, one, one};
+
+  if constexpr (DMA) stage_dy_dma(0, 0); else { load_dy(0); write_dy(0, 0); }
+  load_q(0);
+  write_q(0, 0);
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");          // step s has landed and is written, step s - 1 is read
+    __builtin_amdgcn_s_barrier();
+    const int nb = (s + 1) & 1;
+    const bool more = s + 1 < steps;
+    if (more) {
+      load_q(s + 1);
+      if constexpr (DMA) stage_dy_dma(s + 1, nb); else load_dy(s + 1);
+    }
+    const char* sn = smem + (s & 1) * STAGE;
+    const char* sk = sn + 64 * ROWN;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      bf16x8_t fn[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fn[j] = frag(sn, ROWN, half, wn * TN + j);
+      if (want_db) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fn[j], accb[j], 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < TK; ++i) {
+        const bf16x8_t fk = frag(sk, ROWK, half, wk * TK + i);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fn[j], acc[i][j], 0, 0, 0);
+      }
+    }
+    if (more) {
+      write_q(s + 1, nb);
+      if constexpr (!DMA) write_dy(s + 1, nb);
+    }
+  }
+  float* dw = p.dw + (size_t)blockIdx.y * p.N * p.K;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + (wn * TN + j) * 16 + r16;
+    if (n < p.N) {
+#pragma unroll
+      for (int i = 0; i < TK; ++i) {
+        const int k = k0 + (wk * TK + i) * 16 + g * 4;
+        float* o = dw + (size_t)n * p.K + k;
+        if (k + 4 <= p.K) *reinterpret_cast<w8_f32x4_a4*>(o) = acc[i][j];
+        else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) if (k + e < p.K) o[e] = acc[i][j][e];
+        }
+      }
+      if (want_db && g == 0) p.db[(size_t)blockIdx.y * p.N + n] = accb[j][0];
+    }
+  }
+}
+
+// partial sums [splits][total] -> out [total], in the order of the splits
+__global__ __launch_bounds__(256) void wgrad8_reduce(const float* __restrict__ part, float* __restrict__ out, size_t total, int splits) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= total) return;
+  if (i + 4 <= total) {
+    f32x4_t s = *reinterpret_cast<const w8_f32x4_a4*>(part + i);
+    for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const w8_f32x4_a4*>(part + (size_t)k * total + i);
+    *reinterpret_cast<w8_f32x4_a4*>(out + i) = s;
+  } else {
+    for (size_t e = i; e < total; ++e) {
+      float s = part[e];
+      for (int k = 1; k < splits; ++k) s += part[(size_t)k * total + e];
+      out[e] = s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host entry points
+// ---------------------------------------------------------------------------------------------
+struct W8Plan { bool big; int tiles_n, tiles_k, splits, steps; };
+static W8Plan w8_plan(int T, int N, int K) {
+  W8Plan w;
+  const int kp = b8_kblocks(K) * B8_BLOCK, all = (T + 63) / 64;
+  const long long t256 = (long long)((N + 255) / 256) * ((kp + 255) / 256);
+  w.big = t256 >= 32;
+  const int b = w.big ? 256 : 128;
+  w.tiles_n = (N + b - 1) / b;
+  w.tiles_k = (kp + b - 1) / b;
+  const long long tiles = (long long)w.tiles_n * w.tiles_k, want = w.big ? 256 : 512;
+  // at least 8 steps per split: a split costs a round trip of its partial sums through memory
+  long long splits = want / tiles;
+  if (splits > all / 8) splits = all / 8;
+  if (splits < 1) splits = 1;
+  w.steps = (int)((all + splits - 1) / splits);
+  w.splits = (all + w.steps - 1) / w.steps;
+  return w;
+}
+
+extern "C" size_t sdamd_linear8_weight_grad_ws_bytes(int T, int N, int K) {
+  if (T <= 0 || N <= 0 || K <= 0) return 0;
+  const W8Plan w = w8_plan(T, N, K);
+  return w.splits > 1 ? (size_t)w.splits * ((size_t)N * K + N) * sizeof(float) : 0;
+}
+
+template <int B, int WGN, int WGK, int FMT, bool DMA>
+static int w8_launch(const W8Args& p, int splits, hipStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int lds = 2 * 64 * 2 * B * 2;
+  auto k = wgrad8_kernel<B, B, WGN, WGK, FMT, DMA>;
+  const hipError_t e = sd_lds_opt_in(done, (const void*)k, lds);
+  if (e != hipSuccess) return sdamd_set_error(2, "linear8_weight_grad: %s", hipGetErrorString(e));
+  k<<<dim3(p.tiles_n * p.tiles_k, splits), 64 * WGN * WGK, lds, st>>>(p);
+  return 0;
+}
+
+extern "C" int sdamd_linear8_weight_grad(const void* dy, const void* x8, const unsigned char* x8_scale, float* dw, float* db, void* ws, size_t ws_bytes,
+                                         int T, int N, int K, int fmt, void* stream) {
+  SD_CHECK(fmt == SDAMD_E4M3 || fmt == SDAMD_E5M2, "linear8_weight_grad: unsupported dtype %d", fmt);
+  SD_CHECK(T > 0 && N > 0 && K > 0 && N <= (1 << 30) && K <= (1 << 30) && T <= (1 << 30), "linear8_weight_grad: bad shape T=%d N=%d K=%d", T, N, K);
+  const W8Plan w = w8_plan(T, N, K);
+  SD_CHECK((long long)w.tiles_n * w.tiles_k < (1ll << 31), "linear8_weight_grad: too large, N=%d K=%d", N, K);
+  const size_t need = sdamd_linear8_weight_grad_ws_bytes(T, N, K), nk = (size_t)N * K;
+  SD_CHECK(need == 0 || (ws && ws_bytes >= need), "linear8_weight_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  float* part = (float*)ws;
+  W8Args p{(const bf16_t*)dy, (const unsigned char*)x8, x8_scale, need ? part : dw, db ? (need ? part + w.splits * nk : db) : nullptr,
+           T, N, K, b8_kblocks(K), b8_scale_stride(K), w.tiles_n, w.tiles_k, w.steps};
+  hipStream_t st = (hipStream_t)stream;
+  const bool dma = N % 8 == 0 && ((uintptr_t)dy & 15) == 0;
+  int rc;
+#define W8_FMT(F)                                                                                          \
+  rc = w.big ? (dma ? w8_launch<256, 4, 2, F, true>(p, w.splits, st) : w8_launch<256, 4, 2, F, false>(p, w.splits, st)) \
+             : (dma ? w8_launch<128, 2, 2, F, true>(p, w.splits, st) : w8_launch<128, 2, 2, F, false>(p, w.splits, st))
+  if (fmt == SDAMD_E4M3) W8_FMT(SDAMD_E4M3); else W8_FMT(SDAMD_E5M2);
+#undef W8_FMT
+  if (rc) return rc;
+  SD_LAUNCH_CHECK("linear8_weight_grad");
+  if (need) {
+    wgrad8_reduce<<<(unsigned)((nk + 1023) / 1024), 256, 0, st>>>(part, dw, nk, w.splits);
+    if (db) wgrad8_reduce<<<(N + 1023) / 1024, 256, 0, st>>>(part + w.splits * nk, db, N, w.splits);
+    SD_LAUNCH_CHECK("linear8_weight_grad");
+  }
+  return 0;
+}

@@ -715,3 +715,316 @@ def attention(q, k, v, n_heads, causal=False, out=None):
                                                          _code(q.dtype), _stream())),
            f"B{B} H{n_heads} Sq{Sq} Skv{Skv} d{d}", (2 * B * Sq * C + 2 * B * Skv * C) * q.element_size())
     return out
+
+
+# ------------------------------------------------------------------ 8-bit blocks, and what trains the transformer blocks
+# (diffusion.py:109-137: LayerNorm -> Linear -> GeGLU -> Linear).  Every call may run on any stream and any device its
+# tensors are on; scratch is allocated per call from torch's stream-ordered allocator, so two captured graphs, or two
+# streams, never share it.
+E4M3, E5M2 = 2, 3
+BLOCK8 = 128
+_FMT8 = {torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2}
+
+
+def _need(cond, what, *args):
+    if not cond:
+        raise _lib.SdamdError(what % args if args else what)
+
+
+def _code8(dtype):
+    if dtype not in _FMT8:
+        raise TypeError(f"8-bit blocks are float8_e4m3fn or float8_e5m2, got {dtype}")
+    return _FMT8[dtype]
+
+
+def _call(device, name, *args):
+    """One C-ABI call on the tensors' device and its current stream, whatever the current device is."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _dev8(name, first, *others):
+    """All tensors on one HIP device; returns it."""
+    _dev(first, *others)
+    for t in others:
+        _need(t is None or t.device == first.device, "%s: tensors on %s and %s", name, first.device, t.device if t is not None else "")
+    return first.device
+
+
+def _vec_f32(name, what, t, n):
+    _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, "%s: %s has to be %d contiguous float32 values", name, what, n)
+
+
+class Blocks8:
+    """A matrix in 8-bit blocks: ``q`` [rows, K up to 128] float8_e4m3fn / float8_e5m2 and one power-of-two scale
+    2^(byte - 127) per 128 columns of a row (``block_rows`` = 1: activations, checkpoints) or per 128 x 128 block
+    (``block_rows`` = 128: weights, e4m3), ``scale`` [rows / block_rows, K / 128 up to 4] uint8.  ``shape`` is the shape
+    of the values it stands for.  Made by ``quantize8`` / ``quantize8_weight`` or from stored bytes; columns of ``q``
+    past K have to be zero bytes.  Of an infinity e4m3 keeps NaN, e5m2 keeps it; NaN stays NaN; neither counts for the scale."""
+
+    __slots__ = ("q", "scale", "shape", "block_rows")
+
+    def __init__(self, q, scale, shape, block_rows=1):
+        shape = tuple(int(s) for s in shape)
+        _code8(q.dtype)
+        _need(len(shape) >= 1 and shape[-1] > 0 and block_rows in (1, BLOCK8), "Blocks8: shape %s, block_rows %s", shape, block_rows)
+        rows = 1
+        for s in shape[:-1]:
+            rows *= s
+        kb = -(-shape[-1] // BLOCK8)
+        _need(q.dim() == 2 and tuple(q.shape) == (rows, kb * BLOCK8) and q.is_contiguous(),
+              "Blocks8: q %s has to be a contiguous %s", tuple(q.shape), (rows, kb * BLOCK8))
+        _need(scale.dtype == torch.uint8 and tuple(scale.shape) == (-(-rows // block_rows), -(-kb // 4) * 4) and scale.is_contiguous(),
+              "Blocks8: scale %s %s has to be a contiguous uint8 %s", scale.dtype, tuple(scale.shape), (-(-rows // block_rows), -(-kb // 4) * 4))
+        _need(q.device == scale.device, "Blocks8: q on %s, scale on %s", q.device, scale.device)
+        _need(block_rows == 1 or (q.dtype == torch.float8_e4m3fn and len(shape) == 2), "Blocks8: weights are two-dimensional and float8_e4m3fn")
+        _need(q.data_ptr() % 16 == 0 and scale.data_ptr() % 4 == 0, "Blocks8: q has to be 16-byte aligned, scale 4-byte aligned")
+        self.q, self.scale, self.shape, self.block_rows = q, scale, shape, block_rows
+
+    @property
+    def dtype(self):
+        return self.q.dtype
+
+    @property
+    def device(self):
+        return self.q.device
+
+    @property
+    def nbytes(self):
+        return self.q.numel() + self.scale.numel()
+
+    def dequantize(self, dtype=torch.bfloat16):
+        """The values it stands for; bfloat16 holds every one of them exactly, as float32 does."""
+        dev = _dev8("dequantize", self.q, self.scale)
+        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        code, K = _code(dtype), self.shape[-1]
+        if out.numel():
+            _timed("dequantize8", out.numel() * (1 + out.element_size()),
+                   lambda: _call(dev, "sdamd_dequant8", _p(self.q), _p(self.scale), _p(out), self.q.shape[0], K, self.block_rows,
+                                 _code8(self.dtype), code), f"rows{self.q.shape[0]} K{K}")
+        return out
+
+
+def _blocks8_empty(shape, dtype, device):
+    """Uninitialised activation blocks for the kernels to fill."""
+    rows = 1
+    for s in shape[:-1]:
+        rows *= s
+    kb = -(-shape[-1] // BLOCK8)
+    b = Blocks8.__new__(Blocks8)
+    b.q = torch.empty((rows, kb * BLOCK8), dtype=dtype, device=device)
+    b.scale = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=device)
+    b.shape, b.block_rows = tuple(shape), 1
+    return b
+
+
+def quantize8(x, dtype=torch.float8_e4m3fn):
+    """x [..., K] float32 / bfloat16 (contiguous, or two-dimensional with any row stride) -> Blocks8: per row and 128
+    columns the smallest power-of-two scale that brings the largest magnitude into the type's range, values rounded to
+    nearest even.  The 8-bit operand of ``linear8``, and an activation checkpoint of a quarter / half the bytes."""
+    fmt, code = _code8(dtype), _code(x.dtype)
+    dev = _dev8("quantize8", x)
+    _need(x.dim() >= 1 and x.shape[-1] > 0 and (x.is_contiguous() or (x.dim() == 2 and x.stride(1) == 1)),
+          "quantize8: shape %s, strides %s", tuple(x.shape), tuple(x.stride()))
+    K = x.shape[-1]
+    out = _blocks8_empty(x.shape, dtype, dev)
+    rows = out.q.shape[0]
+    if rows:
+        ldx = K if x.is_contiguous() else x.stride(0)
+        _timed("quantize8", x.numel() * (x.element_size() + 1),
+               lambda: _call(dev, "sdamd_quant8", _p(x), _p(out.q), _p(out.scale), rows, K, ldx, code, fmt), f"rows{rows} K{K}")
+    return out
+
+
+def quantize8_weight(w):
+    """w [N, K] float32 / bfloat16 of any strides -> Blocks8 of 128 x 128 blocks (e4m3), the weight operand of ``linear8``;
+    ``quantize8_weight(w.t())`` is the operand of the gradient with respect to the input."""
+    code = _code(w.dtype)
+    dev = _dev8("quantize8_weight", w)
+    _need(w.dim() == 2 and w.shape[0] > 0 and w.shape[1] > 0, "quantize8_weight: shape %s", tuple(w.shape))
+    N, K = w.shape
+    kb = -(-K // BLOCK8)
+    q = torch.empty((N, kb * BLOCK8), dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty((-(-N // BLOCK8), -(-kb // 4) * 4), dtype=torch.uint8, device=dev)
+    _timed("quantize8_weight", w.numel() * (w.element_size() + 1),
+           lambda: _call(dev, "sdamd_quant8_weight", _p(w), _p(q), _p(scale), N, K, w.stride(0), w.stride(1), code), f"N{N} K{K}")
+    return Blocks8(q, scale, (N, K), BLOCK8)
+
+
+def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=torch.float8_e4m3fn, out=None):
+    """act(x @ w^T + bias + residual) -> [..., N] with both operands in 8-bit blocks: ``w`` from ``quantize8_weight``;
+    ``x`` Blocks8, or float32 / bfloat16 [..., K], then quantised to ``fmt`` on the way (``gemm``'s act: none, quick-gelu,
+    silu).  ``out_dtype`` (default: the residual's, else x's, else bfloat16): a bfloat16 result takes the matrix core's
+    scaled 8-bit products, whose internal sums are good to 1e-5 of the result; a float32 result is summed in float32 from
+    exact products at half that rate."""
+    is8 = isinstance(x, Blocks8)
+    _need(isinstance(w, Blocks8) and w.block_rows == BLOCK8, "linear8: w has to come from quantize8_weight")
+    _need(not is8 or x.block_rows == 1, "linear8: x is a weight")
+    xt = x.q if is8 else x
+    dev = _dev8("linear8", xt, w.q, bias, residual, out)
+    N, K = w.shape
+    _need(len(x.shape) >= 1 and x.shape[-1] == K, "linear8: x %s, w %s", tuple(x.shape), w.shape)
+    if out_dtype is None:
+        out_dtype = residual.dtype if residual is not None else out.dtype if out is not None else torch.bfloat16 if is8 else x.dtype
+    code = _code(out_dtype)
+    _need(act in (ACT_NONE, ACT_QUICK_GELU, ACT_SILU), "linear8: unsupported activation %s", act)
+    shape = tuple(x.shape[:-1]) + (N,)
+    M = 1
+    for s in shape[:-1]:
+        M *= s
+    if bias is not None:
+        _vec_f32("linear8", "bias", bias, N)
+    if residual is not None:
+        _need(residual.dtype == out_dtype and residual.is_contiguous() and tuple(residual.shape) == shape,
+              "linear8: residual %s %s has to be a contiguous %s %s", residual.dtype, tuple(residual.shape), out_dtype, shape)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
+    else:
+        _need(out.dtype == out_dtype and out.is_contiguous() and tuple(out.shape) == shape, "linear8: out %s %s has to be a contiguous %s %s",
+              out.dtype, tuple(out.shape), out_dtype, shape)
+    xcode = f8 = _code8(x.dtype if is8 else fmt)
+    if not is8:
+        xcode = _code(x.dtype)
+    if M == 0:
+        return out
+    if not is8:
+        if M <= _lib.lib().sdamd_linear8_raw_rows() and x.is_contiguous():
+            xp, sp = x, None
+        else:
+            x = quantize8(x, fmt)
+            is8, xcode = True, f8
+    if is8:
+        xp, sp = x.q, x.scale
+    _timed(f"linear8_{_dt(out_dtype)}", 2.0 * M * N * K,
+           lambda: _call(dev, "sdamd_linear8", _p(xp), _p(sp), _p(w.q), _p(w.scale), _p(out), _p(bias), _p(residual), M, N, K,
+                         int(act), xcode, f8, code),
+           f"M{M} N{N} K{K}", M * K * xp.element_size() + N * K + out.numel() * out.element_size() * (1 if residual is None else 2))
+    return out
+
+
+def linear8_weight_grad(dy, x8, bias=True):
+    """Gradient of a Linear's weight and bias from the 8-bit checkpoint of its input: (dw [N, K], db [N] or None), float32,
+    dw = dy^T x8 and db = the sum of dy's rows, for dy [..., N] bfloat16 (contiguous) and ``x8`` = ``quantize8(x)`` (the
+    operand that ``linear8`` took).  Exact products, float32 sums, the same bits every run."""
+    _need(isinstance(x8, Blocks8) and x8.block_rows == 1, "linear8_weight_grad: x8 has to come from quantize8")
+    dev = _dev8("linear8_weight_grad", dy, x8.q)
+    if dy.dtype != torch.bfloat16:
+        raise TypeError(f"linear8_weight_grad: dy has to be bfloat16, got {dy.dtype}")
+    _need(dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape[:-1]) == x8.shape[:-1] and dy.shape[-1] > 0,
+          "linear8_weight_grad: dy %s has to be contiguous beside x8 %s", tuple(dy.shape), x8.shape)
+    N, K, T = dy.shape[-1], x8.shape[-1], x8.q.shape[0]
+    if T == 0:
+        return torch.zeros((N, K), dtype=torch.float32, device=dev), torch.zeros(N, dtype=torch.float32, device=dev) if bias else None
+    dw = torch.empty((N, K), dtype=torch.float32, device=dev)
+    db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
+    need = _lib.lib().sdamd_linear8_weight_grad_ws_bytes(T, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _timed("linear8_weight_grad", 2.0 * T * N * K,
+           lambda: _call(dev, "sdamd_linear8_weight_grad", _p(dy), _p(x8.q), _p(x8.scale), _p(dw), _p(db), _p(ws), need, T, N, K,
+                         _code8(x8.dtype)), f"T{T} N{N} K{K}", 2 * T * N + T * K + 4 * N * K)
+    return dw, db
+
+
+def layernorm_train(x, gamma, beta, eps=1e-5, out_dtype=None):
+    """LayerNorm that keeps what its backward pass needs: (y, mean, rstd) for x [..., C] float32 / bfloat16 contiguous; mean
+    and rstd float32 [rows].  ``out_dtype`` (default: x's): float32, bfloat16, or float8_e4m3fn / float8_e5m2 -- then y is
+    Blocks8, the operand of the following ``linear8`` and its checkpoint, without a pass of its own."""
+    dev = _dev8("layernorm_train", x, gamma, beta)
+    code = _code(x.dtype)
+    _need(x.dim() >= 1 and x.is_contiguous() and x.shape[-1] > 0, "layernorm_train: shape %s, strides %s", tuple(x.shape), tuple(x.stride()))
+    C = x.shape[-1]
+    _vec_f32("layernorm_train", "gamma", gamma, C)
+    _vec_f32("layernorm_train", "beta", beta, C)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    rows = x.numel() // C
+    if out_dtype in _FMT8:
+        y = _blocks8_empty(x.shape, out_dtype, dev)
+        yp, sp, out_code, size = y.q, y.scale, _code8(out_dtype), 1
+    else:
+        out_code = _code(out_dtype)
+        y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+        yp, sp, size = y, None, y.element_size()
+    mean = torch.empty(rows, dtype=torch.float32, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    if rows:
+        _timed("layernorm_train", x.numel() * (x.element_size() + size),
+               lambda: _call(dev, "sdamd_layernorm_train", _p(x), _p(yp), _p(sp), _p(gamma), _p(beta), _p(mean), _p(rstd), rows, C,
+                             float(eps), code, out_code), f"rows{rows} C{C}")
+    return y, mean, rstd
+
+
+def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
+    """Gradients of ``layernorm_train``: (dx, dgamma, dbeta) from dy [..., C] float32 / bfloat16 and the forward pass's x,
+    mean and rstd; ``x`` may be its 8-bit checkpoint (Blocks8).  ``residual`` (dx's shape and type): the gradient that
+    reaches x past the norm (the skip connection), added to dx.  dx has ``out_dtype`` (default: x's type, of a checkpoint
+    the residual's, else dy's); dgamma and dbeta are float32 sums over all rows, the same bits every run."""
+    is8 = isinstance(x, Blocks8)
+    _need(not is8 or x.block_rows == 1, "layernorm_backward: x is a weight")
+    dev = _dev8("layernorm_backward", dy, x.q if is8 else x, gamma, mean, rstd, residual)
+    _need(dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape) == tuple(x.shape) and (is8 or x.is_contiguous()) and dy.shape[-1] > 0,
+          "layernorm_backward: dy %s has to be contiguous beside x %s", tuple(dy.shape), tuple(x.shape))
+    C = dy.shape[-1]
+    rows = dy.numel() // C
+    _vec_f32("layernorm_backward", "gamma", gamma, C)
+    _vec_f32("layernorm_backward", "mean", mean, rows)
+    _vec_f32("layernorm_backward", "rstd", rstd, rows)
+    if out_dtype is None:
+        out_dtype = x.dtype if not is8 else residual.dtype if residual is not None else dy.dtype
+    dcode, xcode, ocode = _code(dy.dtype), _code8(x.dtype) if is8 else _code(x.dtype), _code(out_dtype)
+    if residual is not None:
+        _need(residual.dtype == out_dtype and residual.is_contiguous() and residual.shape == dy.shape,
+              "layernorm_backward: residual %s %s has to be a contiguous %s %s", residual.dtype, tuple(residual.shape), out_dtype, tuple(dy.shape))
+    dx = torch.empty(dy.shape, dtype=out_dtype, device=dev)
+    if rows == 0:
+        return dx, torch.zeros(C, dtype=torch.float32, device=dev), torch.zeros(C, dtype=torch.float32, device=dev)
+    dgamma = torch.empty(C, dtype=torch.float32, device=dev)
+    dbeta = torch.empty(C, dtype=torch.float32, device=dev)
+    need = _lib.lib().sdamd_layernorm_backward_ws_bytes(rows, C)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _timed("layernorm_backward", dy.numel() * (dy.element_size() + (1 if is8 else x.element_size()) + dx.element_size() * (1 if residual is None else 2)),
+           lambda: _call(dev, "sdamd_layernorm_backward", _p(dy), _p(x.q if is8 else x), _p(x.scale if is8 else None), _p(gamma), _p(mean),
+                         _p(rstd), _p(residual), _p(dx), _p(dgamma), _p(dbeta), _p(ws), need, rows, C, dcode, xcode, ocode),
+           f"rows{rows} C{C}")
+    return dx, dgamma, dbeta
+
+
+def geglu_train(h, dtype=torch.float8_e4m3fn):
+    """GeGLU that keeps its input in 8 bits: h [..., 2F] (value | gate) -> (value * gelu(gate) [..., F] in h's type, Blocks8
+    of h), in one pass over h where F is a multiple of 128."""
+    fmt, code = _code8(dtype), _code(h.dtype)
+    dev = _dev8("geglu_train", h)
+    _need(h.dim() >= 1 and h.is_contiguous() and h.shape[-1] > 0 and h.shape[-1] % 2 == 0, "geglu_train: shape %s, strides %s",
+          tuple(h.shape), tuple(h.stride()))
+    Fh = h.shape[-1] // 2
+    out = torch.empty(h.shape[:-1] + (Fh,), dtype=h.dtype, device=dev)
+    kept = _blocks8_empty(h.shape, dtype, dev)
+    rows = kept.q.shape[0]
+    if rows:
+        _timed("geglu_train", h.numel() * (1.5 * h.element_size() + 1),
+               lambda: _call(dev, "sdamd_geglu_train", _p(h), _p(out), _p(kept.q), _p(kept.scale), rows, Fh, code, fmt), f"rows{rows} F{Fh}")
+    return out, kept
+
+
+def geglu_backward(dout, h, out_dtype=None):
+    """Gradient of GeGLU with respect to its input, [..., 2F]: (dout gelu(gate) | dout value gelu'(gate)) from dout [..., F]
+    float32 / bfloat16 and h, the input itself or its 8-bit checkpoint (Blocks8, ``geglu_train``).  ``out_dtype`` default: dout's."""
+    is8 = isinstance(h, Blocks8)
+    _need(not is8 or h.block_rows == 1, "geglu_backward: h is a weight")
+    dev = _dev8("geglu_backward", dout, h.q if is8 else h)
+    _need(dout.dim() >= 1 and dout.is_contiguous() and dout.shape[-1] > 0 and (is8 or h.is_contiguous()) and
+          tuple(h.shape) == tuple(dout.shape[:-1]) + (2 * dout.shape[-1],),
+          "geglu_backward: dout %s has to be contiguous beside h %s", tuple(dout.shape), tuple(h.shape))
+    out_dtype = dout.dtype if out_dtype is None else out_dtype
+    dcode, hcode, ocode = _code(dout.dtype), _code8(h.dtype) if is8 else _code(h.dtype), _code(out_dtype)
+    Fh = dout.shape[-1]
+    rows = dout.numel() // Fh
+    dh = torch.empty(tuple(h.shape), dtype=out_dtype, device=dev)
+    if rows:
+        _timed("geglu_backward", dh.numel() * (dh.element_size() + (1 if is8 else h.element_size()) + dout.element_size() / 2),
+               lambda: _call(dev, "sdamd_geglu_backward", _p(dout), _p(h.q if is8 else h), _p(h.scale if is8 else None), _p(dh), rows, Fh,
+                             dcode, hcode, ocode), f"rows{rows} F{Fh}")
+    return dh

@@ -1,0 +1,83 @@
+"""CPU-only checks of the 8-bit and training operators: arguments are refused before anything is launched, at the C
+boundary and in Python, and the host-side plans hold."""
+import pytest
+import torch
+
+import sd_amd  # noqa: F401
+from sd_amd import _lib, ops
+
+L = _lib.lib()
+P = 4096            # an address that is never read: every call below is refused on the host
+
+
+def refused(rc, text):
+    assert rc != 0 and text in L.sdamd_last_error().decode(), (rc, L.sdamd_last_error())
+
+
+def test_c_boundary_refuses_bad_arguments():
+    refused(L.sdamd_quant8(P, P, P, 0, 5, 5, 0, 2, 0), "bad shape")
+    refused(L.sdamd_quant8(P, P, P, 4, 5, 5, 7, 2, 0), "unsupported dtypes")
+    refused(L.sdamd_quant8(P, P, P, 4, 5, 5, 0, 1, 0), "unsupported dtypes")
+    refused(L.sdamd_quant8(P, P, P, 1 << 40, 1280, 1280, 0, 2, 0), "too large")
+    refused(L.sdamd_quant8_weight(P, P, P, 0, 5, 5, 1, 0, 0), "bad shape")
+    refused(L.sdamd_quant8_weight(P, P, P, 5, 5, -1, 1, 0, 0), "bad shape")
+    refused(L.sdamd_dequant8(P, P, P, 4, 5, 64, 2, 0, 0), "block_rows")
+    refused(L.sdamd_dequant8(P, P, P, 4, 5, 1, 0, 0, 0), "unsupported dtypes")
+    refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 0, 4, 4, 0, 2, 2, 1, 0), "bad shape")
+    refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, 4, 0, 3, 2, 1, 0), "unsupported dtypes")       # blocks of another type than fmt
+    refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 2, 0), "unsupported dtypes")
+    refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, 4, 3, 2, 2, 1, 0), "activation")
+    refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 1, 0), "without their scales")
+    refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, L.sdamd_linear8_raw_rows() + 1, 4, 4, 0, 1, 2, 1, 0), "quantised first")
+    refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 0, 4, 4, 2, 0), "bad shape")
+    refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, 4, 4, 1, 0), "unsupported dtype")
+    need = L.sdamd_linear8_weight_grad_ws_bytes(65536, 320, 320)
+    assert need > 0
+    refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, P, need - 1, 65536, 320, 320, 2, 0), "workspace")
+    refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 4, 12289, 1e-5, 0, 0, 0), "unsupported shape")
+    refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 0, 64, 1e-5, 0, 0, 0), "unsupported shape")
+    refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 4, 64, 1e-5, 0, 2, 0), "without room")
+    refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 4, 64, 1e-5, 2, 0, 0), "unsupported dtypes")
+    need = L.sdamd_layernorm_backward_ws_bytes(4, 64)
+    refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need - 1, 4, 64, 0, 0, 0, 0), "workspace")
+    refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need, 4, 64, 0, 2, 0, 0), "without its scales")
+    refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
+    refused(L.sdamd_geglu_train(P, P, P, P, 0, 64, 0, 2, 0), "bad shape")
+    refused(L.sdamd_geglu_train(P, P, P, P, 4, 64, 2, 2, 0), "unsupported dtypes")
+    refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 0, 2, 0, 0), "without its scales")
+    refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
+
+
+def test_python_refuses_the_cpu_and_bad_blocks():
+    x = torch.zeros(4, 200)
+    for call in (lambda: ops.quantize8(x), lambda: ops.quantize8_weight(x), lambda: ops.layernorm_train(x, x[0], x[0]),
+                 lambda: ops.layernorm_backward(x, x, x[0], x[:, 0], x[:, 0]), lambda: ops.geglu_train(x), lambda: ops.geglu_backward(x[:, :100], x)):
+        with pytest.raises(_lib.SdamdError, match="HIP device"):
+            call()
+    q, s = torch.zeros(4, 256, dtype=torch.float8_e4m3fn), torch.full((4, 4), 127, dtype=torch.uint8)
+    b = ops.Blocks8(q, s, (2, 2, 200))
+    assert b.nbytes == 4 * 256 + 16 and b.dtype == torch.float8_e4m3fn
+    for call in (lambda: b.dequantize(), lambda: ops.geglu_backward(torch.zeros(2, 2, 100), b)):
+        with pytest.raises(_lib.SdamdError, match="HIP device"):
+            call()
+    bad = [(q, s, (4, 257), 1), (q, s, (5, 200), 1), (q[:, :128], s, (4, 128), 1), (q, s[:, :2], (4, 200), 1), (q, s.int(), (4, 200), 1),
+           (q, s, (4, 200), 64), (q, s, (4, 200), 128), (q.view(torch.float8_e5m2), s[:1], (4, 200), 128), (q, s, (4, 0), 1),
+           (torch.zeros(4 * 256 + 16, dtype=torch.uint8)[1:1025].view(torch.float8_e4m3fn).view(4, 256), s, (4, 200), 1)]
+    for args in bad:
+        with pytest.raises(_lib.SdamdError, match="Blocks8"):
+            ops.Blocks8(*args)
+    with pytest.raises(TypeError):
+        ops.Blocks8(q.view(torch.int8), s, (4, 200))
+
+
+def test_workspaces_cover_their_plans():
+    """Few tiles and many tokens are split; wide gradients and short ones are not."""
+    ws = L.sdamd_linear8_weight_grad_ws_bytes
+    assert ws(77, 320, 320) == 0 and ws(0, 4, 4) == 0
+    for t, n, k in ((65536, 320, 320), (16384, 5120, 640), (4099, 333, 215)):
+        per = (n * k + n) * 4
+        assert ws(t, n, k) % per == 0 and ws(t, n, k) // per <= 512
+    for rows, c in ((1, 1), (77, 768), (1 << 30, 320), (4099, 1001), (5, 12288)):      # a row of partial sums per workgroup
+        need = L.sdamd_layernorm_backward_ws_bytes(rows, c)
+        assert need % (8 * c) == 0 and 0 < need <= min(rows, 512) * 8 * c
+    assert L.sdamd_layernorm_backward_ws_bytes(4, 12289) == 0
