@@ -260,11 +260,11 @@ int sdamd_quant8_weight(const void* w, void* q, unsigned char* scale, int N, int
 /* out [rows][K]; block_rows = 1 or 128 (weights) */
 int sdamd_dequant8(const void* q, const unsigned char* scale, void* out, long long rows, int K, int block_rows, int fmt,
                    int out_dtype, void* stream);
-/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n] + residual[m][n]), dense; x: blocks of type fmt (x_dtype == fmt), or at
- * most sdamd_linear8_raw_rows() dense rows of x_dtype F32 / BF16 that the kernel quantises to fmt itself; w: e4m3 weight
- * blocks.  out and residual are out_dtype.  BF16: the scaled 8-bit matrix instruction (its internal sums are good to about
+/* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n] + residual[m][n]), dense; x: blocks of type fmt (x_dtype == fmt), or
+ * -- few of them: where sdamd_linear8_quantises(M, N, K) -- dense rows of x_dtype F32 / BF16 that the kernel quantises to
+ * fmt itself; w: e4m3 weight blocks.  out and residual are out_dtype.  BF16: the scaled 8-bit matrix instruction (its internal sums are good to about
  * 1e-5 of the result); F32: exact products summed in f32 at half the rate.  act: none, quick-gelu, silu. */
-int sdamd_linear8_raw_rows(void);
+int sdamd_linear8_quantises(int M, int N, int K);
 int sdamd_linear8(const void* x, const unsigned char* x_scale, const void* w, const unsigned char* w_scale, void* out,
                   const float* bias, const void* residual, int M, int N, int K, int act, int x_dtype, int fmt,
                   int out_dtype, void* stream);
@@ -278,7 +278,8 @@ int sdamd_linear8_weight_grad(const void* dy, const void* x8, const unsigned cha
 int sdamd_layernorm_train(const void* x, void* y, unsigned char* y_scale, const float* gamma, const float* beta, float* mean,
                           float* rstd, int rows, int C, float eps, int dtype, int out_dtype, void* stream);
 /* its gradients: xh = (x - mean) rstd, a = dy gamma, dx = rstd (a - sum(a)/C - xh sum(a xh)/C) (+ residual, of dx_dtype),
- * dgamma = sum_rows dy xh, dbeta = sum_rows dy (f32, fixed order).  x: F32 / BF16, or row blocks with x_scale. */
+ * dgamma = sum_rows dy xh, dbeta = sum_rows dy (f32, fixed order).  x: F32 / BF16, or row blocks with x_scale.
+ * ws >= sdamd_layernorm_backward_ws_bytes(rows, C), which may be 0. */
 size_t sdamd_layernorm_backward_ws_bytes(int rows, int C);
 int sdamd_layernorm_backward(const void* dy, const void* x, const unsigned char* x_scale, const float* gamma,
                              const float* mean, const float* rstd, const void* residual, void* dx, float* dgamma,

@@ -304,10 +304,18 @@ __global__ __launch_bounds__(512) void gemm8_rows_kernel(G8Args p) {
 // ---------------------------------------------------------------------------------------------
 // host entry points
 // ---------------------------------------------------------------------------------------------
-// rows that sdamd_linear8 quantises itself (x_dtype F32 / BF16): one 16-row tile.  Every workgroup then repeats the
-// quantisation of all rows, which for one tile is cheaper than a launch of its own.
-constexpr int G8_RAW_ROWS = 16;
-extern "C" int sdamd_linear8_raw_rows() { return G8_RAW_ROWS; }
+// Few tiles: the kernel without LDS staging, which also splits K over the waves of a workgroup.
+static bool g8_few_rows(int M, int N) {
+  const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
+  return M <= 64 || (t128 < 96 && (M + 63) / 64 <= 65535);
+}
+// That kernel can quantise rows on its way.  Every workgroup then repeats the work for its rows, so it does where that is
+// cheaper than a launch of its own: up to G8_RAW_WORK values over all workgroups.
+constexpr long long G8_RAW_WORK = 1ll << 24;
+extern "C" int sdamd_linear8_quantises(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return g8_few_rows(M, N) && (long long)((N + 15) / 16) * M <= G8_RAW_WORK / K;
+}
 
 template <int BM, int BN, int WGM, int WGN, int FMT, bool EXACT, typename TO>
 static int g8_tile_launch(G8Args p, hipStream_t st) {
@@ -324,17 +332,20 @@ static int g8_tile_launch(G8Args p, hipStream_t st) {
 
 template <int FMT, bool EXACT, typename TO>
 static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
-  const int nt = (p.N + 15) / 16;
-  if (x_dtype == SDAMD_F32) { gemm8_rows_kernel<1, FMT, EXACT, TO, float><<<dim3(nt, 1), 512, 0, st>>>(p); return 0; }
-  if (x_dtype == SDAMD_BF16) { gemm8_rows_kernel<1, FMT, EXACT, TO, bf16_t><<<dim3(nt, 1), 512, 0, st>>>(p); return 0; }
-  const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256), t128 = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
-  SD_CHECK(t128 < (1ll << 31), "linear8: too large, M=%d N=%d", p.M, p.N);
-  if (p.M <= 64 || (t128 < 96 && (p.M + 63) / 64 <= 65535)) {
-    if (p.M <= 16) gemm8_rows_kernel<1, FMT, EXACT, TO, unsigned char><<<dim3(nt, 1), 512, 0, st>>>(p);
-    else if (p.M <= 32) gemm8_rows_kernel<2, FMT, EXACT, TO, unsigned char><<<dim3(nt, 1), 512, 0, st>>>(p);
-    else gemm8_rows_kernel<4, FMT, EXACT, TO, unsigned char><<<dim3(nt, (p.M + 63) / 64), 512, 0, st>>>(p);
+  if (g8_few_rows(p.M, p.N)) {
+    const dim3 grid((p.N + 15) / 16, p.M <= 32 ? 1 : (p.M + 63) / 64);
+#define G8_ROWS(TX)                                                                              \
+  do {                                                                                           \
+    if (p.M <= 16) gemm8_rows_kernel<1, FMT, EXACT, TO, TX><<<grid, 512, 0, st>>>(p);            \
+    else if (p.M <= 32) gemm8_rows_kernel<2, FMT, EXACT, TO, TX><<<grid, 512, 0, st>>>(p);       \
+    else gemm8_rows_kernel<4, FMT, EXACT, TO, TX><<<grid, 512, 0, st>>>(p);                      \
+  } while (0)
+    if (x_dtype == SDAMD_F32) G8_ROWS(float); else if (x_dtype == SDAMD_BF16) G8_ROWS(bf16_t); else G8_ROWS(unsigned char);
+#undef G8_ROWS
     return 0;
   }
+  const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256), t128 = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
+  SD_CHECK(t128 < (1ll << 31), "linear8: too large, M=%d N=%d", p.M, p.N);
   if constexpr (!EXACT) {
     if (t256 >= 192) return g8_tile_launch<256, 256, 2, 4, FMT, EXACT, TO>(p, st);
   }
@@ -347,7 +358,7 @@ extern "C" int sdamd_linear8(const void* x, const unsigned char* x_scale, const 
            (x_dtype == SDAMD_F32 || x_dtype == SDAMD_BF16 || x_dtype == fmt), "linear8: unsupported dtypes x=%d fmt=%d out=%d", x_dtype, fmt, out_dtype);
   SD_CHECK(M > 0 && N > 0 && K > 0 && N <= (1 << 30) && K <= (1 << 30), "linear8: bad shape M=%d N=%d K=%d", M, N, K);
   SD_CHECK(act == ACT_NONE || act == ACT_QUICK_GELU || act == ACT_SILU, "linear8: unsupported activation %d", act);
-  SD_CHECK(x_dtype >= SDAMD_E4M3 || M <= G8_RAW_ROWS, "linear8: %d rows have to be quantised first (more than %d)", M, G8_RAW_ROWS);
+  SD_CHECK(x_dtype >= SDAMD_E4M3 || sdamd_linear8_quantises(M, N, K), "linear8: M=%d N=%d K=%d: the rows have to be quantised first", M, N, K);
   SD_CHECK(x_dtype < SDAMD_E4M3 || x_scale, "linear8: 8-bit rows without their scales");
   G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0};
   hipStream_t st = (hipStream_t)stream;

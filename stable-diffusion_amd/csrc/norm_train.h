@@ -13,15 +13,17 @@
 
 constexpr int LNT_MAX_C = 256 * 6 * 8;
 
-// sum over the G lanes of a row (G = 256: the whole workgroup, through LDS)
+// sum over the G lanes of a row (G = 256, 512: four or eight waves, through LDS; red: a float per wave of the workgroup)
 template <int G> __device__ __forceinline__ float group_sum(float v, float* red) {
 #pragma unroll
   for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   if constexpr (G > 64) {
+    const int first = G == 256 ? (threadIdx.x >> 8) * 4 : 0;
     __syncthreads();                             // (red may still be read from the previous call)
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (red[0] + red[1]) + (red[2] + red[3]);
+    v = (red[first] + red[first + 1]) + (red[first + 2] + red[first + 3]);
+    if constexpr (G == 512) v += (red[4] + red[5]) + (red[6] + red[7]);
   }
   return v;
 }

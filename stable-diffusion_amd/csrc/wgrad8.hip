@@ -201,18 +201,31 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
   }
 }
 
-// partial sums [splits][total] -> out [total], in the order of the splits
-__global__ __launch_bounds__(256) void wgrad8_reduce(const float* __restrict__ part, float* __restrict__ out, size_t total, int splits) {
-  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+// partial sums -> dw [nk], db [N], in the order of the splits; part: [splits][nk] and behind them [splits][N]
+__global__ __launch_bounds__(256) void wgrad8_reduce(const float* __restrict__ part, float* __restrict__ dw, float* __restrict__ db,
+                                                     size_t nk, int N, int splits, unsigned dw_blocks) {
+  const bool is_b = blockIdx.x >= dw_blocks;
+  const float* src = is_b ? part + splits * nk : part;
+  float* out = is_b ? db : dw;
+  const size_t total = is_b ? (size_t)N : nk;
+  const size_t i = ((size_t)(blockIdx.x - (is_b ? dw_blocks : 0u)) * 256 + threadIdx.x) * 4;
   if (i >= total) return;
   if (i + 4 <= total) {
-    f32x4_t s = *reinterpret_cast<const w8_f32x4_a4*>(part + i);
-    for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const w8_f32x4_a4*>(part + (size_t)k * total + i);
+    f32x4_t s = *reinterpret_cast<const w8_f32x4_a4*>(src + i);
+    int k = 1;
+    for (; k + 4 <= splits; k += 4) {            // four requested at a time
+      f32x4_t v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const w8_f32x4_a4*>(src + (size_t)(k + u) * total + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += v[u];
+    }
+    for (; k < splits; ++k) s += *reinterpret_cast<const w8_f32x4_a4*>(src + (size_t)k * total + i);
     *reinterpret_cast<w8_f32x4_a4*>(out + i) = s;
   } else {
     for (size_t e = i; e < total; ++e) {
-      float s = part[e];
-      for (int k = 1; k < splits; ++k) s += part[(size_t)k * total + e];
+      float s = src[e];
+      for (int k = 1; k < splits; ++k) s += src[(size_t)k * total + e];
       out[e] = s;
     }
   }
@@ -231,9 +244,9 @@ static W8Plan w8_plan(int T, int N, int K) {
   w.tiles_n = (N + b - 1) / b;
   w.tiles_k = (kp + b - 1) / b;
   const long long tiles = (long long)w.tiles_n * w.tiles_k, want = w.big ? 256 : 512;
-  // at least 8 steps per split: a split costs a round trip of its partial sums through memory
+  // at least 2 steps per split: a split costs a round trip of its partial sums through memory
   long long splits = want / tiles;
-  if (splits > all / 8) splits = all / 8;
+  if (splits > all / 2) splits = all / 2;
   if (splits < 1) splits = 1;
   w.steps = (int)((all + splits - 1) / splits);
   w.splits = (all + w.steps - 1) / w.steps;
@@ -279,8 +292,8 @@ extern "C" int sdamd_linear8_weight_grad(const void* dy, const void* x8, const u
   if (rc) return rc;
   SD_LAUNCH_CHECK("linear8_weight_grad");
   if (need) {
-    wgrad8_reduce<<<(unsigned)((nk + 1023) / 1024), 256, 0, st>>>(part, dw, nk, w.splits);
-    if (db) wgrad8_reduce<<<(N + 1023) / 1024, 256, 0, st>>>(part + w.splits * nk, db, N, w.splits);
+    const unsigned dw_blocks = (unsigned)((nk + 1023) / 1024), db_blocks = db ? (N + 1023) / 1024 : 0;
+    wgrad8_reduce<<<dw_blocks + db_blocks, 256, 0, st>>>(part, dw, db, nk, N, w.splits, dw_blocks);
     SD_LAUNCH_CHECK("linear8_weight_grad");
   }
   return 0;

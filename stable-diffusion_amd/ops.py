@@ -7,6 +7,7 @@ launches are capturable into a hipGraph) and never falls back to torch eager mat
 Activation layout is NHWC / token-major: [B, H, W, C] or [B, S, C], float32 or bfloat16.
 """
 import ctypes
+import math
 
 import torch
 
@@ -737,22 +738,31 @@ def _code8(dtype):
     return _FMT8[dtype]
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle without building a Stream object (2 us)
+
+
 def _call(device, name, *args):
     """One C-ABI call on the tensors' device and its current stream, whatever the current device is."""
-    fn = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    fn, i = getattr(_lib.lib(), name), device.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        _lib.check(rc)
 
 
 def _dev8(name, first, *others):
     """All tensors on one HIP device; returns it."""
-    _dev(first, *others)
+    dev = first.device
     for t in others:
-        _need(t is None or t.device == first.device, "%s: tensors on %s and %s", name, first.device, t.device if t is not None else "")
-    return first.device
+        if t is not None and t.device != dev:
+            _dev(first, t)
+            raise _lib.SdamdError(f"{name}: tensors on {dev} and {t.device}")
+    if not first.is_cuda:
+        _dev(first)
+    return dev
 
 
 def _vec_f32(name, what, t, n):
@@ -769,20 +779,22 @@ class Blocks8:
     __slots__ = ("q", "scale", "shape", "block_rows")
 
     def __init__(self, q, scale, shape, block_rows=1):
-        shape = tuple(int(s) for s in shape)
+        shape = tuple(shape)
         _code8(q.dtype)
-        _need(len(shape) >= 1 and shape[-1] > 0 and block_rows in (1, BLOCK8), "Blocks8: shape %s, block_rows %s", shape, block_rows)
-        rows = 1
-        for s in shape[:-1]:
-            rows *= s
-        kb = -(-shape[-1] // BLOCK8)
-        _need(q.dim() == 2 and tuple(q.shape) == (rows, kb * BLOCK8) and q.is_contiguous(),
-              "Blocks8: q %s has to be a contiguous %s", tuple(q.shape), (rows, kb * BLOCK8))
-        _need(scale.dtype == torch.uint8 and tuple(scale.shape) == (-(-rows // block_rows), -(-kb // 4) * 4) and scale.is_contiguous(),
-              "Blocks8: scale %s %s has to be a contiguous uint8 %s", scale.dtype, tuple(scale.shape), (-(-rows // block_rows), -(-kb // 4) * 4))
-        _need(q.device == scale.device, "Blocks8: q on %s, scale on %s", q.device, scale.device)
-        _need(block_rows == 1 or (q.dtype == torch.float8_e4m3fn and len(shape) == 2), "Blocks8: weights are two-dimensional and float8_e4m3fn")
-        _need(q.data_ptr() % 16 == 0 and scale.data_ptr() % 4 == 0, "Blocks8: q has to be 16-byte aligned, scale 4-byte aligned")
+        if len(shape) < 1 or shape[-1] < 1 or min(shape) < 0 or block_rows not in (1, BLOCK8):
+            raise _lib.SdamdError(f"Blocks8: shape {shape}, block_rows {block_rows}")
+        rows, kb = math.prod(shape[:-1]), -(-shape[-1] // BLOCK8)
+        if q.shape != (rows, kb * BLOCK8) or not q.is_contiguous():
+            raise _lib.SdamdError(f"Blocks8: q {tuple(q.shape)} has to be a contiguous {(rows, kb * BLOCK8)}")
+        if scale.dtype != torch.uint8 or scale.shape != (-(-rows // block_rows), -(-kb // 4) * 4) or not scale.is_contiguous():
+            raise _lib.SdamdError(f"Blocks8: scale {scale.dtype} {tuple(scale.shape)} has to be a contiguous uint8 "
+                                  f"{(-(-rows // block_rows), -(-kb // 4) * 4)}")
+        if q.device != scale.device:
+            raise _lib.SdamdError(f"Blocks8: q on {q.device}, scale on {scale.device}")
+        if block_rows != 1 and (q.dtype != torch.float8_e4m3fn or len(shape) != 2):
+            raise _lib.SdamdError("Blocks8: weights are two-dimensional and float8_e4m3fn")
+        if q.data_ptr() % 16 or scale.data_ptr() % 4:
+            raise _lib.SdamdError("Blocks8: q has to be 16-byte aligned, scale 4-byte aligned")
         self.q, self.scale, self.shape, self.block_rows = q, scale, shape, block_rows
 
     @property
@@ -811,10 +823,7 @@ class Blocks8:
 
 def _blocks8_empty(shape, dtype, device):
     """Uninitialised activation blocks for the kernels to fill."""
-    rows = 1
-    for s in shape[:-1]:
-        rows *= s
-    kb = -(-shape[-1] // BLOCK8)
+    rows, kb = math.prod(shape[:-1]), -(-shape[-1] // BLOCK8)
     b = Blocks8.__new__(Blocks8)
     b.q = torch.empty((rows, kb * BLOCK8), dtype=dtype, device=device)
     b.scale = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=device)
@@ -873,9 +882,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     code = _code(out_dtype)
     _need(act in (ACT_NONE, ACT_QUICK_GELU, ACT_SILU), "linear8: unsupported activation %s", act)
     shape = tuple(x.shape[:-1]) + (N,)
-    M = 1
-    for s in shape[:-1]:
-        M *= s
+    M = math.prod(shape[:-1])
     if bias is not None:
         _vec_f32("linear8", "bias", bias, N)
     if residual is not None:
@@ -892,7 +899,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     if M == 0:
         return out
     if not is8:
-        if M <= _lib.lib().sdamd_linear8_raw_rows() and x.is_contiguous():
+        if x.is_contiguous() and _lib.lib().sdamd_linear8_quantises(M, N, K):
             xp, sp = x, None
         else:
             x = quantize8(x, fmt)
@@ -984,7 +991,7 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
     dgamma = torch.empty(C, dtype=torch.float32, device=dev)
     dbeta = torch.empty(C, dtype=torch.float32, device=dev)
     need = _lib.lib().sdamd_layernorm_backward_ws_bytes(rows, C)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _timed("layernorm_backward", dy.numel() * (dy.element_size() + (1 if is8 else x.element_size()) + dx.element_size() * (1 if residual is None else 2)),
            lambda: _call(dev, "sdamd_layernorm_backward", _p(dy), _p(x.q if is8 else x), _p(x.scale if is8 else None), _p(gamma), _p(mean),
                          _p(rstd), _p(residual), _p(dx), _p(dgamma), _p(dbeta), _p(ws), need, rows, C, dcode, xcode, ocode),

@@ -28,7 +28,8 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 2, 0), "unsupported dtypes")
     refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, 4, 3, 2, 2, 1, 0), "activation")
     refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 1, 0), "without their scales")
-    refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, L.sdamd_linear8_raw_rows() + 1, 4, 4, 0, 1, 2, 1, 0), "quantised first")
+    refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 9000, 4096, 4096, 0, 1, 2, 1, 0), "quantised first")
+    assert L.sdamd_linear8_quantises(1, 1280, 320) == 1 and L.sdamd_linear8_quantises(9000, 4096, 4096) == 0 and L.sdamd_linear8_quantises(0, 1, 1) == 0
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 0, 4, 4, 2, 0), "bad shape")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, 4, 4, 1, 0), "unsupported dtype")
     need = L.sdamd_linear8_weight_grad_ws_bytes(65536, 320, 320)
@@ -39,7 +40,8 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 4, 64, 1e-5, 0, 2, 0), "without room")
     refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 4, 64, 1e-5, 2, 0, 0), "unsupported dtypes")
     need = L.sdamd_layernorm_backward_ws_bytes(4, 64)
-    refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need - 1, 4, 64, 0, 0, 0, 0), "workspace")
+    many = L.sdamd_layernorm_backward_ws_bytes(4096, 64)
+    refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, many - 1, 4096, 64, 0, 0, 0, 0), "workspace")
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need, 4, 64, 0, 2, 0, 0), "without its scales")
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
     refused(L.sdamd_geglu_train(P, P, P, P, 0, 64, 0, 2, 0), "bad shape")
@@ -77,7 +79,7 @@ def test_workspaces_cover_their_plans():
     for t, n, k in ((65536, 320, 320), (16384, 5120, 640), (4099, 333, 215)):
         per = (n * k + n) * 4
         assert ws(t, n, k) % per == 0 and ws(t, n, k) // per <= 512
-    for rows, c in ((1, 1), (77, 768), (1 << 30, 320), (4099, 1001), (5, 12288)):      # a row of partial sums per workgroup
+    for rows, c in ((1, 1), (77, 768), (1 << 30, 320), (4099, 1001), (50000, 12288)):  # a row of partial sums per workgroup
         need = L.sdamd_layernorm_backward_ws_bytes(rows, c)
-        assert need % (8 * c) == 0 and 0 < need <= min(rows, 512) * 8 * c
+        assert need % (8 * c) == 0 and need <= min(rows, 512) * 8 * c and (need > 0) == (rows > 1000)
     assert L.sdamd_layernorm_backward_ws_bytes(4, 12289) == 0
