@@ -9,7 +9,6 @@
 // an f32 sum: for an f32 result (EXACT) the bytes and their scales go to bf16, which holds them exactly, and through
 // v_mfma_f32_16x16x32_bf16, whose products and sums are exact to f32 rounding (1.9 PFLOP/s from registers).
 //
-// "A" of the instruction = weight rows, "B" = activation rows: a lane ends up with 4 consecutive columns of one row.
 // Which 32 of a block's 128 values a lane supplies does not matter as long as both operands agree, the scales covering
 // the whole block.
 #include "blocks8.h"
@@ -32,8 +31,8 @@ struct G8Args {
 };
 
 // one 128-wide step of a 16 x 16 tile
-template <int FMT> __device__ __forceinline__ f32x4_t mfma8(i32x8_t w, i32x8_t a, f32x4_t c, int sw, int sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, FMT == SDAMD_E5M2 ? 1 : 0, 0, sw, 0, sa);
+template <int FMT> __device__ __forceinline__ f32x4_t mfma8(i32x8_t a, i32x8_t w, f32x4_t c, int sa, int sw) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, w, c, FMT == SDAMD_E5M2 ? 1 : 0, 0, 0, sa, 0, sw);
 }
 // the EXACT operand: 32 bytes and their scale -> four bf16 fragments
 struct Bf4 { bf16x8_t q[4]; };
@@ -59,25 +58,40 @@ template <int FMT> __device__ __forceinline__ Bf4 to_bf16(i32x8_t v, float s) {
 
 typedef u32x2_t __attribute__((aligned(2))) g8_u32x2_a2;
 typedef f32x4_t __attribute__((aligned(4))) g8_f32x4_a4;
-__device__ __forceinline__ float g8_act(float v, int act) {
-  return act == ACT_SILU ? silu_f(v) : act == ACT_QUICK_GELU ? quick_gelu_f(v) : v;
+// x sigmoid(c x), c = 1 (silu) or 1.702 (quick-gelu); 2^t with what the product t = c x log2(e) lost, so that large |x| keep
+// their digits
+__device__ __forceinline__ float g8_act(float x, int act) {
+  const float z = act == ACT_SILU ? -x : -1.702f * x;
+  const float t = z * 1.44269504f, r = __builtin_fmaf(z, 1.44269504f, -t) + z * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, r * 0.693147181f, e));
 }
+
 // four consecutive columns of row m: + bias + residual, activation, one rounding to the output type
-template <typename TO> __device__ __forceinline__ void g8_store(const G8Args& p, int m, int n, f32x4_t v) {
+__device__ __forceinline__ f32x4_t g8_load4(const float* p) { return *reinterpret_cast<const g8_f32x4_a4*>(p); }
+__device__ __forceinline__ f32x4_t g8_load4(const bf16_t* p) {
+  const u32x2_t t = *reinterpret_cast<const g8_u32x2_a2*>(p);
+  return (f32x4_t){__builtin_bit_cast(float, t[0] << 16), __builtin_bit_cast(float, t[0] & 0xffff0000u),
+                   __builtin_bit_cast(float, t[1] << 16), __builtin_bit_cast(float, t[1] & 0xffff0000u)};
+}
+__device__ __forceinline__ f32x4_t g8_bias4(const G8Args& p, int n) {
+  f32x4_t b = {0.f, 0.f, 0.f, 0.f};
+  if (p.bias) {
+    if (n + 4 <= p.N) b = g8_load4(p.bias + n);
+    else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) if (n + j < p.N) b[j] = p.bias[n + j];
+    }
+  }
+  return b;
+}
+template <typename TO> __device__ __forceinline__ void g8_store4(const G8Args& p, int m, int n, f32x4_t v) {
   if (m >= p.M || n >= p.N) return;
   const size_t at = (size_t)m * p.N + n;
   TO* o = (TO*)p.out + at;
   const TO* r = p.residual ? (const TO*)p.residual + at : nullptr;
   if (n + 4 <= p.N) {
-    if (p.bias) v += *reinterpret_cast<const g8_f32x4_a4*>(p.bias + n);
-    if (r) {
-      if constexpr (sizeof(TO) == 4) v += *reinterpret_cast<const g8_f32x4_a4*>(r);
-      else {
-        const u32x2_t t = *reinterpret_cast<const g8_u32x2_a2*>(r);
-        v += (f32x4_t){__builtin_bit_cast(float, t[0] << 16), __builtin_bit_cast(float, t[0] & 0xffff0000u),
-                       __builtin_bit_cast(float, t[1] << 16), __builtin_bit_cast(float, t[1] & 0xffff0000u)};
-      }
-    }
+    if (r) v += g8_load4(r);
     if (p.act) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = g8_act(v[j], p.act);
@@ -88,134 +102,244 @@ template <typename TO> __device__ __forceinline__ void g8_store(const G8Args& p,
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (n + j < p.N) {
-        float w = v[j];
-        if (p.bias) w += p.bias[n + j];
-        if (r) w += Cvt<TO>::ld(r + j);
-        Cvt<TO>::st(o + j, g8_act(w, p.act));
+        const float w = r ? v[j] + Cvt<TO>::ld(r + j) : v[j];
+        Cvt<TO>::st(o + j, p.act ? g8_act(w, p.act) : w);
       }
   }
 }
 
 // ---- large problems ------------------------------------------------------------------------------------------------
 // Workgroup tile BM x BN, WGM x WGN waves, K step 128 = 128 bytes per row.  Both operands go global -> LDS by
-// global_load_lds_dwordx4 (8 rows of 128 bytes per wave instruction) into two buffers: step t is multiplied while t + 1
-// is on its way.  The 16-byte chunks of a row are permuted by (row >> 1) & 7 on the way in and on the way out, which
-// spreads the rows a fragment read touches over all banks.
-__device__ __forceinline__ void dma16(const void* g, void* lds) {
+// global_load_lds_dwordx4 (8 rows of 128 bytes per wave instruction) into two buffers: step t is multiplied while t + 1 is
+// on its way.  A row's 16-byte chunks are permuted by (row >> 1) & 7 on the way into LDS and out, which spreads a
+// fragment's rows over all banks.
+//
+// "A" of the instruction = activation rows, "B" = weight rows; tile j of a wave's four takes the weight rows 4 r + j (they
+// are put into LDS in that order), so lane r of each 16 ends up with columns 4 r .. 4 r + 3 of one row and the 16 with 64:
+// a store covers whole 128-byte lines from neighbouring lanes.  (With a row per lane, 16 rows x 64 bytes a store, one CU
+// writes 32 GB/s instead of 107, and a 256 x 256 tile takes half as long to store as to multiply at K = 1280.)
+//
+// Workgroups are persistent (PLACES per CU) and run their tiles as one sequence of steps: the first step of the next tile
+// is on its way while the last of this one is multiplied, and its multiplication runs while the stores drain.
+__device__ __forceinline__ void dma16(const void* base, unsigned off, void* lds) {
   // (inline assembly: the builtin makes the compiler wait for all of LDS at every later fragment read; its completion is
   // this kernel's business, s_waitcnt vmcnt(0) and a barrier before the data is read)
   const unsigned l = (unsigned)(unsigned long)(lds_void8_t*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(g) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void* base, unsigned off, void* lds) {
+  const unsigned l = (unsigned)(unsigned long)(lds_void8_t*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
 }
 
 template <int BM, int BN, int WGM, int WGN, int FMT, bool EXACT, typename TO>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
   constexpr int NW = WGM * WGN, TM = BM / WGM / 16, TN = BN / WGN / 16;
-  constexpr int STAGE = (BM + BN) * 128, NI = (BM + BN) / 8 / NW;
-  static_assert((BM + BN) % (8 * NW) == 0 && 128 % (BN / WGN) == 0, "tile shape");
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int STAGE = (BM + BN) * 128, NI = (BM + BN) / 8 / NW;          // DMA instructions of 8 rows per wave and step
+  static_assert((BM + BN) % (8 * NW) == 0 && TN == 4 && BM % 64 == 0 && BM / 64 <= NW && BN / 64 <= NW, "tile shape");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // [2][BM + BN][128] activations, weights | [2][BM] words of four scales | [2][BN] biases
+  char* s_scale = smem + 2 * STAGE;
+  char* s_bias = s_scale + 2 * BM * 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WGN, wn = wave % WGN;
+  const int wm = wave / WGN, wn = wave % WGN, r16 = lane & 15, g = lane >> 4;
+  const int KB = p.KB, ldb = KB * B8_BLOCK;
 
-  // Workgroups go round robin over the 8 XCDs, each with an L2 of its own: give every XCD a run of neighbouring tiles, in
+  // Workgroups go round robin over the 8 XCDs, each with an L2 of its own: every XCD has a run of neighbouring tiles, in
   // groups of 8 row tiles that share their weight tiles.
-  int id = blockIdx.x;
-  {
-    const int total = p.tiles_m * p.tiles_n, per = total / 8, rem = total % 8, x = id % 8, r = id / 8;
-    id = x * per + min(x, rem) + r;
-  }
-  const int group = id / (8 * p.tiles_n), first = group * 8, gm = min(8, p.tiles_m - first), in = id - group * 8 * p.tiles_n;
-  const int m0 = (first + in % gm) * BM, n0 = (in / gm) * BN;
-
-  const unsigned char* src[NI];
-  int dst[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int row = (wave * NI + i) * 8 + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
-    const unsigned char* base = row < BM ? (const unsigned char*)p.A + (size_t)min(m0 + row, p.M - 1) * p.KB * B8_BLOCK
-                                         : p.W + (size_t)min(n0 + row - BM, p.N - 1) * p.KB * B8_BLOCK;
-    src[i] = base + ch * 16;
-    dst[i] = (wave * NI + i) * 1024;
-  }
-  auto stage = [&](int kb, int buf) {
-#pragma unroll
-    for (int i = 0; i < NI; ++i) dma16(src[i] + (size_t)kb * B8_BLOCK, smem + buf * STAGE + dst[i]);
+  const int total = p.tiles_m * p.tiles_n, xcd = blockIdx.x % 8, per = total / 8, rem = total % 8;
+  const int first = xcd * per + min(xcd, rem), count = per + (xcd < rem ? 1 : 0), stride = ((int)gridDim.x - xcd + 7) / 8;
+  int m0 = 0, n0 = 0;
+  auto locate = [&](int id) {
+    const int group = id / (8 * p.tiles_n), fm = group * 8, gm = min(8, p.tiles_m - fm), in = id - group * 8 * p.tiles_n;
+    m0 = (fm + in % gm) * BM;
+    n0 = (in / gm) * BN;
   };
-  // scales: four steps per 32-bit word; a lane holds those of the rows it supplies
-  const unsigned char* sa[TM];
+
+  // per tile: bases (uniform) and the offsets of the rows a lane fetches, held inside the matrix at its edges
+  const unsigned char *baseX = nullptr, *baseS = nullptr, *sw = nullptr;
+  unsigned off[NI], offS = 0;
+  static_assert(BM % (8 * NI) == 0, "a wave fetches rows of one operand");
+  const bool fetches_a = wave * NI * 8 < BM;
+  auto aim = [&]() {
+    baseX = fetches_a ? (const unsigned char*)p.A + (size_t)m0 * ldb : p.W + (size_t)n0 * ldb;
+    baseS = p.As + (size_t)m0 * p.SP;
+    sw = p.Ws + (size_t)(min(n0 + wn * TN * 16, p.N - 1) / B8_BLOCK) * p.SP;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sa[i] = p.As + (size_t)min(m0 + (wm * TM + i) * 16 + (lane & 15), p.M - 1) * p.SP;
-  const unsigned char* sw = p.Ws + (size_t)(min(n0 + wn * TN * 16, p.N - 1) / B8_BLOCK) * p.SP;
-  unsigned sca[TM], scw, nxa[TM], nxw;
+    for (int i = 0; i < NI; ++i) {
+      const int row = (wave * NI + i) * 8 + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
+      const int l = row - BM, wr = (l & ~63) | ((l & 15) << 2) | ((l >> 4) & 3);     // LDS row 64 a + 16 j + r holds weight row 64 a + 4 r + j
+      off[i] = (unsigned)(fetches_a ? min(row, p.M - 1 - m0) : min(wr, p.N - 1 - n0)) * (unsigned)ldb + ch * 16;
+    }
+    offS = (unsigned)min(wave * 64 + lane, p.M - 1 - m0) * (unsigned)p.SP;
+  };
+  unsigned nsw = 0;
+  // request step kb of the tile aimed at into buffer `par` (with step 0 the tile's biases)
+  auto request = [&](int kb, int par, int spar, int bpar) {
+    if (kb == 0 && p.bias && wave < BN / 64)
+      dma4(p.bias + n0, (unsigned)min(wave * 64 + lane, p.N - 1 - n0) * 4u, s_bias + bpar * BN * 4 + wave * 256);
+    const unsigned char* base = baseX + (size_t)kb * B8_BLOCK;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) nxa[i] = *reinterpret_cast<const unsigned*>(sa[i]);
-  nxw = *reinterpret_cast<const unsigned*>(sw);
+    for (int i = 0; i < NI; ++i) dma16(base, off[i], smem + par * STAGE + (wave * NI + i) * 1024);
+    if ((kb & 3) == 0) {
+      if (wave < BM / 64) dma4(baseS + kb, offS, s_scale + spar * BM * 4 + wave * 256);
+      nsw = *reinterpret_cast<const unsigned*>(sw + kb);
+    }
+  };
 
   f32x4_t acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-
-  const int r16 = lane & 15, g = lane >> 4;
-  auto frag = [&](const char* base, int row) {
-    const int o = row * 128 + ((g ^ ((row >> 1) & 7)) << 4);
-    const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(base + o), hi = *reinterpret_cast<const u32x4_t*>(base + (o ^ 64));
+  unsigned sca[TM], scw = 0;
+  // fragment i of the rows from LDS offset `at` on: tile rows are 2 KB apart, the permutation depends on the lane alone
+  const unsigned in_row = r16 * 128 + ((g ^ (r16 >> 1)) << 4), at_a = wm * TM * 2048 + in_row, at_w = BM * 128 + wn * TN * 2048 + in_row;
+  auto frag = [&](unsigned at, int i) {
+    const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(smem + at + i * 2048), hi = *reinterpret_cast<const u32x4_t*>(smem + (at ^ 64u) + i * 2048);
     return (i32x8_t){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   };
-
-  stage(0, 0);
-  for (int kb = 0; kb < p.KB; ++kb) {
-    // step kb has landed (it was issued a whole step ago), and this wave's reads of step kb - 1 are done
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  auto multiply = [&](int kb, int par, int spar) {
+    const unsigned a0 = at_a + par * STAGE, w0 = at_w + par * STAGE;
     if ((kb & 3) == 0) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) { asm volatile("" : "+v"(nxa[i])); sca[i] = nxa[i]; }   // (used here, where nothing is in flight)
-      asm volatile("" : "+v"(nxw));
-      scw = nxw;
+      for (int i = 0; i < TM; ++i) sca[i] = *reinterpret_cast<const unsigned*>(s_scale + (spar * BM + (wm * TM + i) * 16 + r16) * 4);
     }
-    __builtin_amdgcn_s_barrier();
-    if (kb + 1 < p.KB) stage(kb + 1, (kb + 1) & 1);
-    if ((kb & 3) == 3 && kb + 1 < p.KB) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) nxa[i] = *reinterpret_cast<const unsigned*>(sa[i] + kb + 1);
-      nxw = *reinterpret_cast<const unsigned*>(sw + kb + 1);
-    }
-    const char* sA = smem + (kb & 1) * STAGE;
-    const char* sW = sA + BM * 128;
-    const int sh = (kb & 3) * 8;
-    const int bw = (int)(scw >> sh);
+    const int sh = (kb & 3) * 8, bw = (int)(scw >> sh);
     if constexpr (!EXACT) {
-      i32x8_t w[TN];
+      i32x8_t wc[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) w[j] = frag(sW, (wn * TN + j) * 16 + r16);
+      for (int j = 0; j < TN; ++j) wc[j] = frag(w0, j);
+      // activation fragments are read AHEAD tiles ahead of their use; left alone the compiler requests all of them first,
+      // for which there are no registers beside the sums
+      constexpr int AHEAD = 2;
+      i32x8_t a[AHEAD + 1];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) a[i] = frag(a0, i);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const i32x8_t a = frag(sA, (wm * TM + i) * 16 + r16);
+        if (i + AHEAD < TM) a[(i + AHEAD) % (AHEAD + 1)] = frag(a0, i + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
         const int ba = (int)(sca[i] >> sh);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma8<FMT>(w[j], a, acc[i][j], bw, ba);
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma8<FMT>(a[i % (AHEAD + 1)], wc[j], acc[i][j], ba, bw);
       }
     } else {
       Bf4 w[TN];
       const float fw = b8_scale(bw & 255);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) w[j] = to_bf16<SDAMD_E4M3>(frag(sW, (wn * TN + j) * 16 + r16), fw);
+      for (int j = 0; j < TN; ++j) w[j] = to_bf16<SDAMD_E4M3>(frag(w0, j), fw);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const Bf4 a = to_bf16<FMT>(frag(sA, (wm * TM + i) * 16 + r16), b8_scale((int)(sca[i] >> sh) & 255));
+        const Bf4 a = to_bf16<FMT>(frag(a0, i), b8_scale((int)(sca[i] >> sh) & 255));
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j].q[q], a.q[q], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.q[q], w[j].q[q], acc[i][j], 0, 0, 0);
       }
     }
+  };
+  // A store is a uniform row address and a lane offset that all of the tile's rows share; inside the matrix without tests,
+  // at its edges under a mask; the residual and the activation have a loop of their own.  (With tests of everything at every
+  // store, the two waves of a SIMD spent 10 us of instructions on a 256 x 256 tile, of which the stores themselves are 2.)
+  auto store = [&](int tm0, int tn0, int bpar) {
+    const int n = tn0 + wn * 64 + r16 * 4;
+    int left = p.M - (tm0 + wm * TM * 16 + g * 4);         // rows from the lane's first one to the end
+    f32x4_t bias = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias) bias = *reinterpret_cast<const f32x4_t*>(s_bias + bpar * BN * 4 + (wn * 64 + r16 * 4) * 4);
+    auto value = [&](int i, int e) { return (f32x4_t){acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]} + bias; };
+    // (or the compiler adds the bias to the whole tile before it branches, in registers of their own)
+    auto branch = [&]() { asm volatile("" : "+v"(bias)); };
+    const size_t ld = (size_t)p.N * sizeof(TO), at = (size_t)(tm0 + wm * TM * 16) * ld + (size_t)tn0 * sizeof(TO);
+    char* out = (char*)p.out + at;
+    const char* res = p.residual ? (const char*)p.residual + at : nullptr;
+    const unsigned lo = (unsigned)(g * 4) * (unsigned)ld + (unsigned)(wn * 64 + r16 * 4) * (unsigned)sizeof(TO);
+    auto put = [&](f32x4_t v) {
+      if constexpr (sizeof(TO) == 4) *reinterpret_cast<g8_f32x4_a4*>(out + lo) = v;
+      else *reinterpret_cast<g8_u32x2_a2*>(out + lo) = (u32x2_t){pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
+    };
+    // the next row; the assembly keeps the compiler from working out all rows' addresses ahead of time (registers)
+    auto down = [&](int e) {
+      out += e == 3 ? 13 * ld : ld;
+      asm volatile("" : "+s"(out));
+      if (res) {
+        res += e == 3 ? 13 * ld : ld;
+        asm volatile("" : "+s"(res));
+      }
+    };
+    if (!res && !p.act && tm0 + BM <= p.M && tn0 + BN <= p.N) {
+      branch();
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { put(value(i, e)); down(e); }
+      return;
+    }
+    branch();
+    const int cols = p.N - n;                              // of the lane's four (<= 0: none)
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      asm volatile("" : "+v"(left));                       // (32 masks at once would take 64 scalar registers)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f32x4_t v = value(i, e);
+        if (e < left && cols > 0) {
+          const TO* r = (const TO*)(res + lo);
+          TO* o = (TO*)(out + lo);
+          if (res) {
+            if (cols >= 4) v += g8_load4(r);
+            else {
+#pragma unroll
+              for (int j = 0; j < 3; ++j) if (j < cols) v[j] += Cvt<TO>::ld(r + j);
+            }
+          }
+          if (p.act) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = g8_act(v[j], p.act);
+          }
+          if (cols >= 4) put(v);
+          else {
+#pragma unroll
+            for (int j = 0; j < 3; ++j) if (j < cols) Cvt<TO>::st(o + j, v[j]);
+          }
+        }
+        down(e);
+      }
+      left -= 16;
+    }
+  };
+
+  int t = blockIdx.x / 8;
+  if (t >= count) return;
+  locate(first + t);
+  aim();
+  request(0, 0, 0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  int par = 0, spar = 0, bpar = 0;                         // buffers of the step, of its group of four scales, of the tile's biases
+  while (true) {
+    const int tm0 = m0, tn0 = n0;
+    t += stride;
+    const bool more = t < count;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int kb = 0; kb < KB; ++kb) {
+      __builtin_amdgcn_s_barrier();                        // everyone's part of step kb is in LDS, everyone is done with the other buffer
+      if ((kb & 3) == 0) scw = nsw;
+      const bool last = kb + 1 == KB;
+      const int nspar = (kb & 3) == 3 || last ? spar ^ 1 : spar;
+      if (last && more) {
+        locate(first + t);
+        aim();
+      }
+      if (!last || more) request(last ? 0 : kb + 1, par ^ 1, nspar, bpar ^ 1);
+      multiply(kb, par, spar);
+      // what the wave requested has landed and its LDS reads are done
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      par ^= 1;
+      spar = nspar;
+    }
+    store(tm0, tn0, bpar);
+    if (!more) return;
+    bpar ^= 1;
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-      g8_store<TO>(p, m0 + (wm * TM + i) * 16 + r16, n0 + (wn * TN + j) * 16 + g * 4, acc[i][j]);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
@@ -278,26 +402,28 @@ __global__ __launch_bounds__(512) void gemm8_rows_kernel(G8Args p) {
     const i32x8_t w = {(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
     if constexpr (!EXACT) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = mfma8<FMT>(w, a[i], acc[i], bw, ba[i]);
+      for (int i = 0; i < MT; ++i) acc[i] = mfma8<FMT>(a[i], w, acc[i], ba[i], bw);
     } else {
       const Bf4 wb = to_bf16<SDAMD_E4M3>(w, b8_scale(bw));
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const Bf4 ab = to_bf16<FMT>(a[i], b8_scale(ba[i]));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb.q[q], ab.q[q], acc[i], 0, 0, 0);
+        for (int q = 0; q < 4; ++q) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ab.q[q], wb.q[q], acc[i], 0, 0, 0);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4_t*>(&ex[wave][i * 16 + r16][g * 4]) = acc[i];
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ex[wave][i * 16 + g * 4 + e][r16] = acc[i][e];
   __syncthreads();
   for (int t = threadIdx.x; t < MT * 64; t += 512) {
     const int row = t >> 2, c = (t & 3) * 4;
     f32x4_t s = *reinterpret_cast<const f32x4_t*>(&ex[0][row][c]);
 #pragma unroll
     for (int w = 1; w < 8; ++w) s += *reinterpret_cast<const f32x4_t*>(&ex[w][row][c]);
-    g8_store<TO>(p, m0 + row, n0 + c, s);
+    g8_store4<TO>(p, m0 + row, n0 + c, s + g8_bias4(p, n0 + c));
   }
 }
 
@@ -311,22 +437,25 @@ static bool g8_few_rows(int M, int N) {
 }
 // That kernel can quantise rows on its way.  Every workgroup then repeats the work for its rows, so it does where that is
 // cheaper than a launch of its own: up to G8_RAW_WORK values over all workgroups.
+#ifndef G8_T256
+#define G8_T256 192
+#endif
 constexpr long long G8_RAW_WORK = 1ll << 24;
 extern "C" int sdamd_linear8_quantises(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   return g8_few_rows(M, N) && (long long)((N + 15) / 16) * M <= G8_RAW_WORK / K;
 }
 
-template <int BM, int BN, int WGM, int WGN, int FMT, bool EXACT, typename TO>
+template <int BM, int BN, int WGM, int WGN, int PLACES, int FMT, bool EXACT, typename TO>
 static int g8_tile_launch(G8Args p, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  constexpr int lds = 2 * (BM + BN) * 128;
+  constexpr int lds = 2 * ((BM + BN) * 128 + BM * 4) + 2 * BN * 4;
   auto k = gemm8_kernel<BM, BN, WGM, WGN, FMT, EXACT, TO>;
   const hipError_t e = sd_lds_opt_in(done, (const void*)k, lds);
   if (e != hipSuccess) return sdamd_set_error(2, "linear8: %s", hipGetErrorString(e));
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
-  k<<<p.tiles_m * p.tiles_n, 64 * WGM * WGN, lds, st>>>(p);
+  k<<<min(p.tiles_m * p.tiles_n, 256 * PLACES), 64 * WGM * WGN, lds, st>>>(p);
   return 0;
 }
 
@@ -347,9 +476,9 @@ static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
   const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256), t128 = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
   SD_CHECK(t128 < (1ll << 31), "linear8: too large, M=%d N=%d", p.M, p.N);
   if constexpr (!EXACT) {
-    if (t256 >= 192) return g8_tile_launch<256, 256, 2, 4, FMT, EXACT, TO>(p, st);
+    if (t256 >= G8_T256) return g8_tile_launch<256, 256, 2, 4, 1, FMT, EXACT, TO>(p, st);
   }
-  return g8_tile_launch<128, 128, 2, 2, FMT, EXACT, TO>(p, st);
+  return g8_tile_launch<128, 128, 2, 2, 2, FMT, EXACT, TO>(p, st);
 }
 
 extern "C" int sdamd_linear8(const void* x, const unsigned char* x_scale, const void* w, const unsigned char* w_scale, void* out, const float* bias,
