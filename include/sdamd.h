@@ -261,10 +261,10 @@ int sdamd_quant8_weight(const void* w, void* q, unsigned char* scale, int N, int
 int sdamd_dequant8(const void* q, const unsigned char* scale, void* out, long long rows, int K, int block_rows, int fmt,
                    int out_dtype, void* stream);
 /* out[m][n] = act(sum_k x[m][k] w[n][k] + bias[n] + residual[m][n]), dense; x: blocks of type fmt (x_dtype == fmt), or
- * -- few of them: where sdamd_linear8_quantises(M, N, K) -- dense rows of x_dtype F32 / BF16 that the kernel quantises to
+ * -- few of them: where sdamd_linear8_quantises(M, N, K, out_dtype) -- dense rows of x_dtype F32 / BF16 that the kernel quantises to
  * fmt itself; w: e4m3 weight blocks.  out and residual are out_dtype.  BF16: the scaled 8-bit matrix instruction (its internal sums are good to about
  * 1e-5 of the result); F32: exact products summed in f32 at half the rate.  act: none, quick-gelu, silu. */
-int sdamd_linear8_quantises(int M, int N, int K);
+int sdamd_linear8_quantises(int M, int N, int K, int out_dtype);
 int sdamd_linear8(const void* x, const unsigned char* x_scale, const void* w, const unsigned char* w_scale, void* out,
                   const float* bias, const void* residual, int M, int N, int K, int act, int x_dtype, int fmt,
                   int out_dtype, void* stream);

@@ -58,7 +58,7 @@ SIGNATURES = {
     "sdamd_quant8": (_i, [_vp, _vp, _vp, _ll, _i, _ll, _i, _i, _vp]),
     "sdamd_quant8_weight": (_i, [_vp, _vp, _vp, _i, _i, _ll, _ll, _i, _vp]),
     "sdamd_dequant8": (_i, [_vp, _vp, _vp, _ll, _i, _i, _i, _i, _vp]),
-    "sdamd_linear8_quantises": (_i, [_i, _i, _i]),
+    "sdamd_linear8_quantises": (_i, [_i, _i, _i, _i]),
     "sdamd_linear8": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
     "sdamd_linear8_weight_grad_ws_bytes": (_sz, [_i, _i, _i]),
     "sdamd_linear8_weight_grad": (_i, [_vp] * 6 + [_sz] + [_i] * 4 + [_vp]),

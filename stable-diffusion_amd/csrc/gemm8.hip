@@ -351,7 +351,7 @@ __global__ __launch_bounds__(512) void gemm8_rows_kernel(G8Args p) {
   constexpr bool XRAW = sizeof(TX) != 1;
   constexpr int LD = 20;                                   // floats per row of the exchange: 16 columns, 16-byte aligned
   __shared__ __attribute__((aligned(16))) float ex[8][MT * 16][LD];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
   const unsigned char* wr = p.W + (size_t)min(n0 + r16, p.N - 1) * p.KB * B8_BLOCK + g * 32;
   const unsigned char* sw = p.Ws + (size_t)(n0 / B8_BLOCK) * p.SP;
@@ -430,20 +430,19 @@ __global__ __launch_bounds__(512) void gemm8_rows_kernel(G8Args p) {
 // ---------------------------------------------------------------------------------------------
 // host entry points
 // ---------------------------------------------------------------------------------------------
-// Few tiles: the kernel without LDS staging, which also splits K over the waves of a workgroup.
-static bool g8_few_rows(int M, int N) {
-  const long long t128 = (long long)((M + 127) / 128) * ((N + 127) / 128);
-  return M <= 64 || (t128 < 96 && (M + 63) / 64 <= 65535);
+// Few tiles: the kernel without LDS staging, which also splits K over the waves of a workgroup.  The tile kernel takes
+// 0.65 us a step with few tiles on the chip, 1.3 us in its f32 form (512 x 1280 -> 1280, 40 tiles: 9.3 us, this one 12.0;
+// 20 tiles: 9.1 and 8.6; f32 80 tiles: 16.7 and 22.9, 48 tiles: 8.0 and 6.3).
+static long long g8_tiles(int M, int N, int b) { return (long long)((M + b - 1) / b) * ((N + b - 1) / b); }
+static bool g8_few_rows(int M, int N, bool exact) {
+  return M <= 64 || (g8_tiles(M, N, 128) < (exact ? 64 : 32) && (M + 63) / 64 <= 65535);
 }
 // That kernel can quantise rows on its way.  Every workgroup then repeats the work for its rows, so it does where that is
 // cheaper than a launch of its own: up to G8_RAW_WORK values over all workgroups.
-#ifndef G8_T256
-#define G8_T256 192
-#endif
 constexpr long long G8_RAW_WORK = 1ll << 24;
-extern "C" int sdamd_linear8_quantises(int M, int N, int K) {
+extern "C" int sdamd_linear8_quantises(int M, int N, int K, int out_dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return g8_few_rows(M, N) && (long long)((N + 15) / 16) * M <= G8_RAW_WORK / K;
+  return g8_few_rows(M, N, out_dtype == SDAMD_F32) && (long long)((N + 15) / 16) * M <= G8_RAW_WORK / K;
 }
 
 template <int BM, int BN, int WGM, int WGN, int PLACES, int FMT, bool EXACT, typename TO>
@@ -461,7 +460,7 @@ static int g8_tile_launch(G8Args p, hipStream_t st) {
 
 template <int FMT, bool EXACT, typename TO>
 static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
-  if (g8_few_rows(p.M, p.N)) {
+  if (g8_few_rows(p.M, p.N, EXACT)) {
     const dim3 grid((p.N + 15) / 16, p.M <= 32 ? 1 : (p.M + 63) / 64);
 #define G8_ROWS(TX)                                                                              \
   do {                                                                                           \
@@ -473,10 +472,12 @@ static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
 #undef G8_ROWS
     return 0;
   }
-  const long long t256 = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256), t128 = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
-  SD_CHECK(t128 < (1ll << 31), "linear8: too large, M=%d N=%d", p.M, p.N);
+  SD_CHECK(g8_tiles(p.M, p.N, 128) < (1ll << 31), "linear8: too large, M=%d N=%d", p.M, p.N);
+  // 256 x 256 where it fills the chip and does not multiply an eighth more padding than 128 x 128 (two workgroups per CU):
+  // 65536 x 320 -> 2560: 92 us, with 128 x 128 129; -> 320 (512 columns instead of 384): 23.7 and 19.5.  f32: 128 x 128.
   if constexpr (!EXACT) {
-    if (t256 >= G8_T256) return g8_tile_launch<256, 256, 2, 4, 1, FMT, EXACT, TO>(p, st);
+    const long long t = g8_tiles(p.M, p.N, 256);
+    if (t >= 192 && t * 4 * 8 <= g8_tiles(p.M, p.N, 128) * 9) return g8_tile_launch<256, 256, 2, 4, 1, FMT, EXACT, TO>(p, st);
   }
   return g8_tile_launch<128, 128, 2, 2, 2, FMT, EXACT, TO>(p, st);
 }
@@ -487,7 +488,7 @@ extern "C" int sdamd_linear8(const void* x, const unsigned char* x_scale, const 
            (x_dtype == SDAMD_F32 || x_dtype == SDAMD_BF16 || x_dtype == fmt), "linear8: unsupported dtypes x=%d fmt=%d out=%d", x_dtype, fmt, out_dtype);
   SD_CHECK(M > 0 && N > 0 && K > 0 && N <= (1 << 30) && K <= (1 << 30), "linear8: bad shape M=%d N=%d K=%d", M, N, K);
   SD_CHECK(act == ACT_NONE || act == ACT_QUICK_GELU || act == ACT_SILU, "linear8: unsupported activation %d", act);
-  SD_CHECK(x_dtype >= SDAMD_E4M3 || sdamd_linear8_quantises(M, N, K), "linear8: M=%d N=%d K=%d: the rows have to be quantised first", M, N, K);
+  SD_CHECK(x_dtype >= SDAMD_E4M3 || sdamd_linear8_quantises(M, N, K, out_dtype), "linear8: M=%d N=%d K=%d: the rows have to be quantised first", M, N, K);
   SD_CHECK(x_dtype < SDAMD_E4M3 || x_scale, "linear8: 8-bit rows without their scales");
   G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0};
   hipStream_t st = (hipStream_t)stream;

@@ -899,7 +899,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     if M == 0:
         return out
     if not is8:
-        if x.is_contiguous() and _lib.lib().sdamd_linear8_quantises(M, N, K):
+        if x.is_contiguous() and _lib.lib().sdamd_linear8_quantises(M, N, K, code):
             xp, sp = x, None
         else:
             x = quantize8(x, fmt)

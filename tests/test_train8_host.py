@@ -29,7 +29,7 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, 4, 3, 2, 2, 1, 0), "activation")
     refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 1, 0), "without their scales")
     refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 9000, 4096, 4096, 0, 1, 2, 1, 0), "quantised first")
-    assert L.sdamd_linear8_quantises(1, 1280, 320) == 1 and L.sdamd_linear8_quantises(9000, 4096, 4096) == 0 and L.sdamd_linear8_quantises(0, 1, 1) == 0
+    assert L.sdamd_linear8_quantises(1, 1280, 320, 1) == 1 and L.sdamd_linear8_quantises(9000, 4096, 4096, 1) == 0 and L.sdamd_linear8_quantises(0, 1, 1, 0) == 0
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 0, 4, 4, 2, 0), "bad shape")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, 4, 4, 1, 0), "unsupported dtype")
     need = L.sdamd_linear8_weight_grad_ws_bytes(65536, 320, 320)
