@@ -13,6 +13,7 @@
 // in a fixed order (no atomics: the same bits every run).
 #include "blocks8.h"
 #include "gemm_common.h"
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) void lds_voidw_t;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2w_t;
@@ -70,70 +71,101 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
   const int t_begin = blockIdx.y * p.steps * 64, t_end = min(p.T, t_begin + p.steps * 64);
   const int steps = (t_end - t_begin + 63) / 64;           // (the launcher leaves no split empty)
 
-  auto stage_dy_dma = [&](int s, int buf) {
+  // Pieces of 16 bytes: a thread's places in the tiles are the same every step, so are its offsets from the step's first
+  // token.  Columns past N or the row's last block are taken from inside the row (they only reach results that are not
+  // stored); tokens past the end are zeros in both operands.
+  const char* dy0 = reinterpret_cast<const char*>(p.dy) + (size_t)t_begin * p.N * 2;
+  const unsigned char* q0 = p.q + (size_t)t_begin * p.KB * B8_BLOCK;
+  const unsigned char* s0 = p.qs + (size_t)t_begin * p.SP;
+  unsigned off_d[DI], off_q[QI], off_s[QI];
+  int shift_s[QI];
 #pragma unroll
-    for (int i = 0; i < DI; ++i) {
-      const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-      const int col = (((c >> 1) ^ w8_swz(t)) * 2 + (c & 1)) * 8;       // column whose 16 bytes belong at this place
-      const int tok = t_begin + s * 64 + t;
-      const void* src = tok < t_end && n0 + col < p.N ? (const void*)(p.dy + (size_t)tok * p.N + n0 + col) : (const void*)g_wgrad_zero;
-      const unsigned l = (unsigned)(unsigned long)(lds_voidw_t*)(smem + buf * STAGE + (i * NT + (tid & ~63)) * 16);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(src) : "memory", "m0");
-    }
-  };
+  for (int i = 0; i < DI; ++i) {
+    const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
+    const int col = n0 + (DMA ? ((c >> 1) ^ w8_swz(t)) * 2 + (c & 1) : c) * 8;          // (DMA: the column whose 16 bytes belong at this place)
+    off_d[i] = (unsigned)t * (unsigned)p.N * 2u + (unsigned)(DMA ? min(col, p.N - 8) : col) * 2u;
+  }
+#pragma unroll
+  for (int i = 0; i < QI; ++i) {
+    const int piece = i * NT + tid, t = piece / (BT_K / 16), kc = min(k0 + piece % (BT_K / 16) * 16, p.KB * B8_BLOCK - 16);
+    off_q[i] = (unsigned)t * (unsigned)(p.KB * B8_BLOCK) + (unsigned)kc;
+    off_s[i] = (unsigned)t * (unsigned)p.SP + (unsigned)(kc / B8_BLOCK & ~3);           // (the word with the scale; a byte load's
+    shift_s[i] = (kc / B8_BLOCK & 3) * 8;                                               //  extension the compiler would wait for at once)
+  }
   Raw8<bf16_t> rd[DMA ? 1 : DI];
-  auto load_dy = [&](int s) {
-#pragma unroll
-    for (int i = 0; i < DI; ++i) {
-      const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-      rd[DMA ? 0 : i] = raw8_load(p.dy + (size_t)min(t_begin + s * 64 + t, p.T - 1) * p.N, n0 + c * 8, p.N);
-    }
-  };
-  auto write_dy = [&](int s, int buf) {
-#pragma unroll
-    for (int i = 0; i < DI; ++i) {
-      const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-      float v[8];
-      raw8_get(rd[DMA ? 0 : i], n0 + c * 8, p.N, v);
-      u32x4_t o = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
-      if (t_begin + s * 64 + t >= t_end) o = (u32x4_t){0u, 0u, 0u, 0u};
-      *reinterpret_cast<u32x4_t*>(smem + buf * STAGE + t * ROWN + (((c >> 1) ^ w8_swz(t)) * 2 + (c & 1)) * 16) = o;
-    }
-  };
   u32x4_t rq[QI];
-  int rs[QI];
-  auto load_q = [&](int s) {
+  unsigned rs[QI];
+  auto request = [&](int s, int buf) {
+    const int left = t_end - (t_begin + s * 64);           // tokens from the step's first one to the end
+    const unsigned char* q = q0 + (size_t)s * 64 * p.KB * B8_BLOCK;
+    const unsigned char* sc = s0 + (size_t)s * 64 * p.SP;
+    const char* d = dy0 + (size_t)s * 64 * p.N * 2;
 #pragma unroll
     for (int i = 0; i < QI; ++i) {
-      const int piece = i * NT + tid, t = piece / (BT_K / 16), u = piece % (BT_K / 16);
-      const size_t tok = min(t_begin + s * 64 + t, p.T - 1);
-      const int kc = min(k0 + u * 16, p.KB * B8_BLOCK - 16);            // (columns past the row: some of it, never stored)
-      rq[i] = *reinterpret_cast<const u32x4_t*>(p.q + tok * p.KB * B8_BLOCK + kc);
-      rs[i] = p.qs[tok * p.SP + kc / B8_BLOCK];
+      const bool in = (i * NT + tid) / (BT_K / 16) < left;
+      rq[i] = *reinterpret_cast<const u32x4_t*>(q + (in ? off_q[i] : 0u));
+      rs[i] = *reinterpret_cast<const unsigned*>(sc + (in ? off_s[i] : 0u));
+    }
+    auto place = [&](int i) {
+      return __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(lds_voidw_t*)(smem + buf * STAGE + (i * NT + (tid & ~63)) * 16));
+    };
+    if constexpr (DMA) {
+      if (left >= 64) {
+#pragma unroll
+        for (int i = 0; i < DI; ++i)
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place(i)), "v"(off_d[i]), "s"(d) : "memory", "m0");
+      } else {
+#pragma unroll
+        for (int i = 0; i < DI; ++i) {
+          const void* src = (i * NT + tid) / (ROWN / 16) < left ? (const void*)(d + off_d[i]) : (const void*)g_wgrad_zero;
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(place(i)), "v"(src) : "memory", "m0");
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < DI; ++i) {
+        const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
+        rd[DMA ? 0 : i] = raw8_load(reinterpret_cast<const bf16_t*>(d) + (size_t)min(t, left - 1) * p.N, n0 + c * 8, p.N);
+      }
     }
   };
-  auto write_q = [&](int s, int buf) {
+  // what came through registers goes to LDS
+  auto write = [&](int s, int buf) {
+    const int left = t_end - (t_begin + s * 64);
 #pragma unroll
     for (int i = 0; i < QI; ++i) {
       const int piece = i * NT + tid, t = piece / (BT_K / 16), u = piece % (BT_K / 16);
       u32x4_t lo, hi;
-      w8_to_bf16<FMT>(rq[i], b8_scale(rs[i]), lo, hi);
-      if (t_begin + s * 64 + t >= t_end) { lo = (u32x4_t){0u, 0u, 0u, 0u}; hi = lo; }
+      w8_to_bf16<FMT>(rq[i], b8_scale((int)(rs[i] >> shift_s[i]) & 255), lo, hi);
+      if (t >= left) { lo = (u32x4_t){0u, 0u, 0u, 0u}; hi = lo; }
       char* d = smem + buf * STAGE + 64 * ROWN + t * ROWK + ((u ^ w8_swz(t)) << 5);
       *reinterpret_cast<u32x4_t*>(d) = lo;
       *reinterpret_cast<u32x4_t*>(d + 16) = hi;
     }
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int i = 0; i < DI; ++i) {
+        const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
+        float v[8];
+        raw8_get(rd[DMA ? 0 : i], n0 + c * 8, p.N, v);
+        u32x4_t o = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
+        if (t >= left) o = (u32x4_t){0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4_t*>(smem + buf * STAGE + t * ROWN + (((c >> 1) ^ w8_swz(t)) * 2 + (c & 1)) * 16) = o;
+      }
+    }
   };
-  // 8 tokens (8 g .. of a 32-token half) of the 16 columns of unit u
-  auto frag = [&](const char* base, int row_bytes, int half, int u) {
+  // 8 tokens (8 g .. of a 32-token half) of the 16 columns of unit u.  A lane's address: its token and place in the unit,
+  // and the unit's place u ^ f, of which the low three bits are permuted and f (the same for t and t + 4) is the lane's own.
+  const int f_t = w8_swz(g * 8 + (r16 >> 2));
+  auto frag = [&](unsigned at, int row_bytes, int half, int u) {
     typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
-    const int t = half * 32 + g * 8 + (r16 >> 2), f = w8_swz(t);        // (t and t + 4 have the same f)
-    const char* a = base + t * row_bytes + ((u ^ f) << 5) + (r16 & 3) * 8;
+    const char* a = smem + at + half * 32 * row_bytes + ((u ^ f_t) << 5);
     const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)a);
     const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(a + 4 * row_bytes));
     typedef __attribute__((ext_vector_type(8))) short s16x8_t;
     return __builtin_bit_cast(bf16x8_t, (s16x8_t){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   };
+  const unsigned lane_n = (g * 8 + (r16 >> 2)) * ROWN + (r16 & 3) * 8, lane_k = 64 * ROWN + (g * 8 + (r16 >> 2)) * ROWK + (r16 & 3) * 8;
 
   f32x4_t acc[TK][TN], accb[TN];
 #pragma unroll
@@ -146,41 +178,42 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
   const __bf16 one = (__bf16)1.0f;
   const bf16x8_t ones = {one, one, one, one, one, one, one, one};
 
-  if constexpr (DMA) stage_dy_dma(0, 0); else { load_dy(0); write_dy(0, 0); }
-  load_q(0);
-  write_q(0, 0);
-  for (int s = 0; s < steps; ++s) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");          // step s has landed and is written, step s - 1 is read
-    __builtin_amdgcn_s_barrier();
-    const int nb = (s + 1) & 1;
-    const bool more = s + 1 < steps;
-    if (more) {
-      load_q(s + 1);
-      if constexpr (DMA) stage_dy_dma(s + 1, nb); else load_dy(s + 1);
-    }
-    const char* sn = smem + (s & 1) * STAGE;
-    const char* sk = sn + 64 * ROWN;
+  // (two loops: a test of want_db inside would make the compiler move all sums around it)
+  auto run = [&](auto with_db) {
+    request(0, 0);
+    write(0, 0);
+#pragma unroll 1
+    for (int s = 0; s < steps; ++s) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");        // step s has landed and is written, step s - 1 is read
+      __builtin_amdgcn_s_barrier();
+      const bool more = s + 1 < steps;
+      if (more) request(s + 1, (s + 1) & 1);
+      const unsigned an = lane_n + (s & 1) * STAGE, ak = lane_k + (s & 1) * STAGE;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      bf16x8_t fn[TN];
+      for (int half = 0; half < 2; ++half) {
+        bf16x8_t fn[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fn[j] = frag(sn, ROWN, half, wn * TN + j);
-      if (want_db) {
+        for (int j = 0; j < TN; ++j) fn[j] = frag(an, ROWN, half, wn * TN + j);
+        if constexpr (decltype(with_db)::value) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fn[j], accb[j], 0, 0, 0);
+          for (int j = 0; j < TN; ++j) accb[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, fn[j], accb[j], 0, 0, 0);
+        }
+        constexpr int AHEAD = 2;                 // k fragments are read this many tiles ahead of their use
+        bf16x8_t fk[AHEAD + 1];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fk[i] = frag(ak, ROWK, half, wk * TK + i);
+#pragma unroll
+        for (int i = 0; i < TK; ++i) {
+          if (i + AHEAD < TK) fk[(i + AHEAD) % (AHEAD + 1)] = frag(ak, ROWK, half, wk * TK + i + AHEAD);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk[i % (AHEAD + 1)], fn[j], acc[i][j], 0, 0, 0);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < TK; ++i) {
-        const bf16x8_t fk = frag(sk, ROWK, half, wk * TK + i);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fk, fn[j], acc[i][j], 0, 0, 0);
-      }
+      if (more) write(s + 1, (s + 1) & 1);
     }
-    if (more) {
-      write_q(s + 1, nb);
-      if constexpr (!DMA) write_dy(s + 1, nb);
-    }
-  }
+  };
+  if (want_db) run(std::true_type{}); else run(std::false_type{});
   float* dw = p.dw + (size_t)blockIdx.y * p.N * p.K;
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
