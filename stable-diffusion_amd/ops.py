@@ -738,13 +738,14 @@ def _code8(dtype):
     return _FMT8[dtype]
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle without building a Stream object (2 us)
+# the current device's number and a stream's handle without the Python objects around them (2 us a call)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _call(device, name, *args):
+def _call(device, name, args):
     """One C-ABI call on the tensors' device and its current stream, whatever the current device is."""
     fn, i = getattr(_lib.lib(), name), device.index
-    if i == torch.cuda.current_device():
+    if i == _current_device():
         rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(device):
@@ -753,16 +754,25 @@ def _call(device, name, *args):
         _lib.check(rc)
 
 
+def _run8(device, name, args, label):
+    """``_call``, timed where a profiler is on; ``label()`` gives _timed's (kind, work, shape, bytes)."""
+    if PROFILER is None:
+        _call(device, name, args)
+    else:
+        kind, work, shape, nbytes = label()
+        _timed(kind, work, lambda: _call(device, name, args), shape, nbytes)
+
+
 def _dev8(name, first, *others):
     """All tensors on one HIP device; returns it."""
-    dev = first.device
+    i = first.get_device()
     for t in others:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != i:
             _dev(first, t)
-            raise _lib.SdamdError(f"{name}: tensors on {dev} and {t.device}")
-    if not first.is_cuda:
+            raise _lib.SdamdError(f"{name}: tensors on {first.device} and {t.device}")
+    if i < 0:
         _dev(first)
-    return dev
+    return first.device
 
 
 def _vec_f32(name, what, t, n):
@@ -815,9 +825,8 @@ class Blocks8:
         out = torch.empty(self.shape, dtype=dtype, device=dev)
         code, K = _code(dtype), self.shape[-1]
         if out.numel():
-            _timed("dequantize8", out.numel() * (1 + out.element_size()),
-                   lambda: _call(dev, "sdamd_dequant8", _p(self.q), _p(self.scale), _p(out), self.q.shape[0], K, self.block_rows,
-                                 _code8(self.dtype), code), f"rows{self.q.shape[0]} K{K}")
+            _run8(dev, "sdamd_dequant8", (_p(self.q), _p(self.scale), _p(out), self.q.shape[0], K, self.block_rows, _code8(self.dtype), code),
+                  lambda: ("dequantize8", out.numel() * (1 + out.element_size()), f"rows{self.q.shape[0]} K{K}", 0.0))
         return out
 
 
@@ -837,15 +846,15 @@ def quantize8(x, dtype=torch.float8_e4m3fn):
     nearest even.  The 8-bit operand of ``linear8``, and an activation checkpoint of a quarter / half the bytes."""
     fmt, code = _code8(dtype), _code(x.dtype)
     dev = _dev8("quantize8", x)
-    _need(x.dim() >= 1 and x.shape[-1] > 0 and (x.is_contiguous() or (x.dim() == 2 and x.stride(1) == 1)),
-          "quantize8: shape %s, strides %s", tuple(x.shape), tuple(x.stride()))
+    if not (x.dim() >= 1 and x.shape[-1] > 0 and (x.is_contiguous() or (x.dim() == 2 and x.stride(1) == 1))):
+        raise _lib.SdamdError("quantize8: shape %s, strides %s" % (tuple(x.shape), tuple(x.stride())))
     K = x.shape[-1]
     out = _blocks8_empty(x.shape, dtype, dev)
     rows = out.q.shape[0]
     if rows:
         ldx = K if x.is_contiguous() else x.stride(0)
-        _timed("quantize8", x.numel() * (x.element_size() + 1),
-               lambda: _call(dev, "sdamd_quant8", _p(x), _p(out.q), _p(out.scale), rows, K, ldx, code, fmt), f"rows{rows} K{K}")
+        _run8(dev, "sdamd_quant8", (_p(x), _p(out.q), _p(out.scale), rows, K, ldx, code, fmt),
+              lambda: ("quantize8", x.numel() * (x.element_size() + 1), f"rows{rows} K{K}", 0.0))
     return out
 
 
@@ -854,13 +863,14 @@ def quantize8_weight(w):
     ``quantize8_weight(w.t())`` is the operand of the gradient with respect to the input."""
     code = _code(w.dtype)
     dev = _dev8("quantize8_weight", w)
-    _need(w.dim() == 2 and w.shape[0] > 0 and w.shape[1] > 0, "quantize8_weight: shape %s", tuple(w.shape))
+    if not (w.dim() == 2 and w.shape[0] > 0 and w.shape[1] > 0):
+        raise _lib.SdamdError("quantize8_weight: shape %s" % (tuple(w.shape),))
     N, K = w.shape
     kb = -(-K // BLOCK8)
     q = torch.empty((N, kb * BLOCK8), dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty((-(-N // BLOCK8), -(-kb // 4) * 4), dtype=torch.uint8, device=dev)
-    _timed("quantize8_weight", w.numel() * (w.element_size() + 1),
-           lambda: _call(dev, "sdamd_quant8_weight", _p(w), _p(q), _p(scale), N, K, w.stride(0), w.stride(1), code), f"N{N} K{K}")
+    _run8(dev, "sdamd_quant8_weight", (_p(w), _p(q), _p(scale), N, K, w.stride(0), w.stride(1), code),
+          lambda: ("quantize8_weight", w.numel() * (w.element_size() + 1), f"N{N} K{K}", 0.0))
     return Blocks8(q, scale, (N, K), BLOCK8)
 
 
@@ -871,28 +881,31 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     scaled 8-bit products, whose internal sums are good to 1e-5 of the result; a float32 result is summed in float32 from
     exact products at half that rate."""
     is8 = isinstance(x, Blocks8)
-    _need(isinstance(w, Blocks8) and w.block_rows == BLOCK8, "linear8: w has to come from quantize8_weight")
-    _need(not is8 or x.block_rows == 1, "linear8: x is a weight")
+    if not (isinstance(w, Blocks8) and w.block_rows == BLOCK8):
+        raise _lib.SdamdError("linear8: w has to come from quantize8_weight")
+    if is8 and x.block_rows != 1:
+        raise _lib.SdamdError("linear8: x is a weight")
     xt = x.q if is8 else x
     dev = _dev8("linear8", xt, w.q, bias, residual, out)
     N, K = w.shape
-    _need(len(x.shape) >= 1 and x.shape[-1] == K, "linear8: x %s, w %s", tuple(x.shape), w.shape)
+    if not (len(x.shape) >= 1 and x.shape[-1] == K):
+        raise _lib.SdamdError("linear8: x %s, w %s" % (tuple(x.shape), w.shape))
     if out_dtype is None:
         out_dtype = residual.dtype if residual is not None else out.dtype if out is not None else torch.bfloat16 if is8 else x.dtype
     code = _code(out_dtype)
-    _need(act in (ACT_NONE, ACT_QUICK_GELU, ACT_SILU), "linear8: unsupported activation %s", act)
+    if act not in (ACT_NONE, ACT_QUICK_GELU, ACT_SILU):
+        raise _lib.SdamdError("linear8: unsupported activation %s" % (act,))
     shape = tuple(x.shape[:-1]) + (N,)
     M = math.prod(shape[:-1])
     if bias is not None:
         _vec_f32("linear8", "bias", bias, N)
     if residual is not None:
-        _need(residual.dtype == out_dtype and residual.is_contiguous() and tuple(residual.shape) == shape,
-              "linear8: residual %s %s has to be a contiguous %s %s", residual.dtype, tuple(residual.shape), out_dtype, shape)
+        if not (residual.dtype == out_dtype and residual.is_contiguous() and tuple(residual.shape) == shape):
+            raise _lib.SdamdError("linear8: residual %s %s has to be a contiguous %s %s" % (residual.dtype, tuple(residual.shape), out_dtype, shape))
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=dev)
-    else:
-        _need(out.dtype == out_dtype and out.is_contiguous() and tuple(out.shape) == shape, "linear8: out %s %s has to be a contiguous %s %s",
-              out.dtype, tuple(out.shape), out_dtype, shape)
+    elif not (out.dtype == out_dtype and out.is_contiguous() and tuple(out.shape) == shape):
+        raise _lib.SdamdError("linear8: out %s %s has to be a contiguous %s %s" % (out.dtype, tuple(out.shape), out_dtype, shape))
     xcode = f8 = _code8(x.dtype if is8 else fmt)
     if not is8:
         xcode = _code(x.dtype)
@@ -906,10 +919,9 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
             is8, xcode = True, f8
     if is8:
         xp, sp = x.q, x.scale
-    _timed(f"linear8_{_dt(out_dtype)}", 2.0 * M * N * K,
-           lambda: _call(dev, "sdamd_linear8", _p(xp), _p(sp), _p(w.q), _p(w.scale), _p(out), _p(bias), _p(residual), M, N, K,
-                         int(act), xcode, f8, code),
-           f"M{M} N{N} K{K}", M * K * xp.element_size() + N * K + out.numel() * out.element_size() * (1 if residual is None else 2))
+    _run8(dev, "sdamd_linear8", (_p(xp), _p(sp), _p(w.q), _p(w.scale), _p(out), _p(bias), _p(residual), M, N, K, int(act), xcode, f8, code),
+          lambda: (f"linear8_{_dt(out_dtype)}", 2.0 * M * N * K, f"M{M} N{N} K{K}",
+                   M * K * xp.element_size() + N * K + out.numel() * out.element_size() * (1 if residual is None else 2)))
     return out
 
 
@@ -917,12 +929,13 @@ def linear8_weight_grad(dy, x8, bias=True):
     """Gradient of a Linear's weight and bias from the 8-bit checkpoint of its input: (dw [N, K], db [N] or None), float32,
     dw = dy^T x8 and db = the sum of dy's rows, for dy [..., N] bfloat16 (contiguous) and ``x8`` = ``quantize8(x)`` (the
     operand that ``linear8`` took).  Exact products, float32 sums, the same bits every run."""
-    _need(isinstance(x8, Blocks8) and x8.block_rows == 1, "linear8_weight_grad: x8 has to come from quantize8")
+    if not (isinstance(x8, Blocks8) and x8.block_rows == 1):
+        raise _lib.SdamdError("linear8_weight_grad: x8 has to come from quantize8")
     dev = _dev8("linear8_weight_grad", dy, x8.q)
     if dy.dtype != torch.bfloat16:
         raise TypeError(f"linear8_weight_grad: dy has to be bfloat16, got {dy.dtype}")
-    _need(dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape[:-1]) == x8.shape[:-1] and dy.shape[-1] > 0,
-          "linear8_weight_grad: dy %s has to be contiguous beside x8 %s", tuple(dy.shape), x8.shape)
+    if not (dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape[:-1]) == x8.shape[:-1] and dy.shape[-1] > 0):
+        raise _lib.SdamdError("linear8_weight_grad: dy %s has to be contiguous beside x8 %s" % (tuple(dy.shape), x8.shape))
     N, K, T = dy.shape[-1], x8.shape[-1], x8.q.shape[0]
     if T == 0:
         return torch.zeros((N, K), dtype=torch.float32, device=dev), torch.zeros(N, dtype=torch.float32, device=dev) if bias else None
@@ -930,9 +943,8 @@ def linear8_weight_grad(dy, x8, bias=True):
     db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
     need = _lib.lib().sdamd_linear8_weight_grad_ws_bytes(T, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _timed("linear8_weight_grad", 2.0 * T * N * K,
-           lambda: _call(dev, "sdamd_linear8_weight_grad", _p(dy), _p(x8.q), _p(x8.scale), _p(dw), _p(db), _p(ws), need, T, N, K,
-                         _code8(x8.dtype)), f"T{T} N{N} K{K}", 2 * T * N + T * K + 4 * N * K)
+    _run8(dev, "sdamd_linear8_weight_grad", (_p(dy), _p(x8.q), _p(x8.scale), _p(dw), _p(db), _p(ws), need, T, N, K, _code8(x8.dtype)),
+          lambda: ("linear8_weight_grad", 2.0 * T * N * K, f"T{T} N{N} K{K}", 2 * T * N + T * K + 4 * N * K))
     return dw, db
 
 
@@ -942,7 +954,8 @@ def layernorm_train(x, gamma, beta, eps=1e-5, out_dtype=None):
     Blocks8, the operand of the following ``linear8`` and its checkpoint, without a pass of its own."""
     dev = _dev8("layernorm_train", x, gamma, beta)
     code = _code(x.dtype)
-    _need(x.dim() >= 1 and x.is_contiguous() and x.shape[-1] > 0, "layernorm_train: shape %s, strides %s", tuple(x.shape), tuple(x.stride()))
+    if not (x.dim() >= 1 and x.is_contiguous() and x.shape[-1] > 0):
+        raise _lib.SdamdError("layernorm_train: shape %s, strides %s" % (tuple(x.shape), tuple(x.stride())))
     C = x.shape[-1]
     _vec_f32("layernorm_train", "gamma", gamma, C)
     _vec_f32("layernorm_train", "beta", beta, C)
@@ -958,9 +971,8 @@ def layernorm_train(x, gamma, beta, eps=1e-5, out_dtype=None):
     mean = torch.empty(rows, dtype=torch.float32, device=dev)
     rstd = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows:
-        _timed("layernorm_train", x.numel() * (x.element_size() + size),
-               lambda: _call(dev, "sdamd_layernorm_train", _p(x), _p(yp), _p(sp), _p(gamma), _p(beta), _p(mean), _p(rstd), rows, C,
-                             float(eps), code, out_code), f"rows{rows} C{C}")
+        _run8(dev, "sdamd_layernorm_train", (_p(x), _p(yp), _p(sp), _p(gamma), _p(beta), _p(mean), _p(rstd), rows, C, float(eps), code, out_code),
+              lambda: ("layernorm_train", x.numel() * (x.element_size() + size), f"rows{rows} C{C}", 0.0))
     return y, mean, rstd
 
 
@@ -970,10 +982,11 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
     reaches x past the norm (the skip connection), added to dx.  dx has ``out_dtype`` (default: x's type, of a checkpoint
     the residual's, else dy's); dgamma and dbeta are float32 sums over all rows, the same bits every run."""
     is8 = isinstance(x, Blocks8)
-    _need(not is8 or x.block_rows == 1, "layernorm_backward: x is a weight")
+    if is8 and x.block_rows != 1:
+        raise _lib.SdamdError("layernorm_backward: x is a weight")
     dev = _dev8("layernorm_backward", dy, x.q if is8 else x, gamma, mean, rstd, residual)
-    _need(dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape) == tuple(x.shape) and (is8 or x.is_contiguous()) and dy.shape[-1] > 0,
-          "layernorm_backward: dy %s has to be contiguous beside x %s", tuple(dy.shape), tuple(x.shape))
+    if not (dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape) == tuple(x.shape) and (is8 or x.is_contiguous()) and dy.shape[-1] > 0):
+        raise _lib.SdamdError("layernorm_backward: dy %s has to be contiguous beside x %s" % (tuple(dy.shape), tuple(x.shape)))
     C = dy.shape[-1]
     rows = dy.numel() // C
     _vec_f32("layernorm_backward", "gamma", gamma, C)
@@ -983,8 +996,8 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
         out_dtype = x.dtype if not is8 else residual.dtype if residual is not None else dy.dtype
     dcode, xcode, ocode = _code(dy.dtype), _code8(x.dtype) if is8 else _code(x.dtype), _code(out_dtype)
     if residual is not None:
-        _need(residual.dtype == out_dtype and residual.is_contiguous() and residual.shape == dy.shape,
-              "layernorm_backward: residual %s %s has to be a contiguous %s %s", residual.dtype, tuple(residual.shape), out_dtype, tuple(dy.shape))
+        if not (residual.dtype == out_dtype and residual.is_contiguous() and residual.shape == dy.shape):
+            raise _lib.SdamdError("layernorm_backward: residual %s %s has to be a contiguous %s %s" % (residual.dtype, tuple(residual.shape), out_dtype, tuple(dy.shape)))
     dx = torch.empty(dy.shape, dtype=out_dtype, device=dev)
     if rows == 0:
         return dx, torch.zeros(C, dtype=torch.float32, device=dev), torch.zeros(C, dtype=torch.float32, device=dev)
@@ -992,10 +1005,10 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
     dbeta = torch.empty(C, dtype=torch.float32, device=dev)
     need = _lib.lib().sdamd_layernorm_backward_ws_bytes(rows, C)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _timed("layernorm_backward", dy.numel() * (dy.element_size() + (1 if is8 else x.element_size()) + dx.element_size() * (1 if residual is None else 2)),
-           lambda: _call(dev, "sdamd_layernorm_backward", _p(dy), _p(x.q if is8 else x), _p(x.scale if is8 else None), _p(gamma), _p(mean),
-                         _p(rstd), _p(residual), _p(dx), _p(dgamma), _p(dbeta), _p(ws), need, rows, C, dcode, xcode, ocode),
-           f"rows{rows} C{C}")
+    _run8(dev, "sdamd_layernorm_backward", (_p(dy), _p(x.q if is8 else x), _p(x.scale if is8 else None), _p(gamma), _p(mean), _p(rstd),
+                                            _p(residual), _p(dx), _p(dgamma), _p(dbeta), _p(ws), need, rows, C, dcode, xcode, ocode),
+          lambda: ("layernorm_backward", dy.numel() * (dy.element_size() + (1 if is8 else x.element_size()) +
+                                                       dx.element_size() * (1 if residual is None else 2)), f"rows{rows} C{C}", 0.0))
     return dx, dgamma, dbeta
 
 
@@ -1004,15 +1017,15 @@ def geglu_train(h, dtype=torch.float8_e4m3fn):
     of h), in one pass over h where F is a multiple of 128."""
     fmt, code = _code8(dtype), _code(h.dtype)
     dev = _dev8("geglu_train", h)
-    _need(h.dim() >= 1 and h.is_contiguous() and h.shape[-1] > 0 and h.shape[-1] % 2 == 0, "geglu_train: shape %s, strides %s",
-          tuple(h.shape), tuple(h.stride()))
+    if not (h.dim() >= 1 and h.is_contiguous() and h.shape[-1] > 0 and h.shape[-1] % 2 == 0):
+        raise _lib.SdamdError("geglu_train: shape %s, strides %s" % (tuple(h.shape), tuple(h.stride())))
     Fh = h.shape[-1] // 2
     out = torch.empty(h.shape[:-1] + (Fh,), dtype=h.dtype, device=dev)
     kept = _blocks8_empty(h.shape, dtype, dev)
     rows = kept.q.shape[0]
     if rows:
-        _timed("geglu_train", h.numel() * (1.5 * h.element_size() + 1),
-               lambda: _call(dev, "sdamd_geglu_train", _p(h), _p(out), _p(kept.q), _p(kept.scale), rows, Fh, code, fmt), f"rows{rows} F{Fh}")
+        _run8(dev, "sdamd_geglu_train", (_p(h), _p(out), _p(kept.q), _p(kept.scale), rows, Fh, code, fmt),
+              lambda: ("geglu_train", h.numel() * (1.5 * h.element_size() + 1), f"rows{rows} F{Fh}", 0.0))
     return out, kept
 
 
@@ -1020,18 +1033,18 @@ def geglu_backward(dout, h, out_dtype=None):
     """Gradient of GeGLU with respect to its input, [..., 2F]: (dout gelu(gate) | dout value gelu'(gate)) from dout [..., F]
     float32 / bfloat16 and h, the input itself or its 8-bit checkpoint (Blocks8, ``geglu_train``).  ``out_dtype`` default: dout's."""
     is8 = isinstance(h, Blocks8)
-    _need(not is8 or h.block_rows == 1, "geglu_backward: h is a weight")
+    if is8 and h.block_rows != 1:
+        raise _lib.SdamdError("geglu_backward: h is a weight")
     dev = _dev8("geglu_backward", dout, h.q if is8 else h)
-    _need(dout.dim() >= 1 and dout.is_contiguous() and dout.shape[-1] > 0 and (is8 or h.is_contiguous()) and
-          tuple(h.shape) == tuple(dout.shape[:-1]) + (2 * dout.shape[-1],),
-          "geglu_backward: dout %s has to be contiguous beside h %s", tuple(dout.shape), tuple(h.shape))
+    if not (dout.dim() >= 1 and dout.is_contiguous() and dout.shape[-1] > 0 and (is8 or h.is_contiguous()) and tuple(h.shape) == tuple(dout.shape[:-1]) + (2 * dout.shape[-1],)):
+        raise _lib.SdamdError("geglu_backward: dout %s has to be contiguous beside h %s" % (tuple(dout.shape), tuple(h.shape)))
     out_dtype = dout.dtype if out_dtype is None else out_dtype
     dcode, hcode, ocode = _code(dout.dtype), _code8(h.dtype) if is8 else _code(h.dtype), _code(out_dtype)
     Fh = dout.shape[-1]
     rows = dout.numel() // Fh
     dh = torch.empty(tuple(h.shape), dtype=out_dtype, device=dev)
     if rows:
-        _timed("geglu_backward", dh.numel() * (dh.element_size() + (1 if is8 else h.element_size()) + dout.element_size() / 2),
-               lambda: _call(dev, "sdamd_geglu_backward", _p(dout), _p(h.q if is8 else h), _p(h.scale if is8 else None), _p(dh), rows, Fh,
-                             dcode, hcode, ocode), f"rows{rows} F{Fh}")
+        _run8(dev, "sdamd_geglu_backward", (_p(dout), _p(h.q if is8 else h), _p(h.scale if is8 else None), _p(dh), rows, Fh, dcode, hcode, ocode),
+              lambda: ("geglu_backward", dh.numel() * (dh.element_size() + (1 if is8 else h.element_size()) + dout.element_size() / 2),
+                       f"rows{rows} F{Fh}", 0.0))
     return dh
