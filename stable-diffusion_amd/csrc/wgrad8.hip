@@ -268,22 +268,32 @@ __global__ __launch_bounds__(256) void wgrad8_reduce(const float* __restrict__ p
 // host entry points
 // ---------------------------------------------------------------------------------------------
 struct W8Plan { bool big; int tiles_n, tiles_k, splits, steps; };
+// Tile size and number of splits by the least estimated time, in us, from what the kernels measured: a step of 64 tokens
+// takes 1.67 with one 256 x 256 workgroup on a CU, 0.8 with one of 128 x 128 and 1.17 with two; a split result costs its
+// partial sums' way through memory (both ways at 4 TB/s) and a launch.  16384 x 5120 x 640: 60 large tiles in 4 splits
+// 140 us (3: 174, 6: 182; 200 small tiles in 4: 166); 65536 x 320 x 320: small in 48, 42 us (large in 64: 51);
+// 1024 x 1280 x 1280: small, not split, 19.8 us (in 2: 22.1; large in 6: 29.1).
 static W8Plan w8_plan(int T, int N, int K) {
-  W8Plan w;
+  static const int tries[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 56, 64, 80, 96, 112, 128};
   const int kp = b8_kblocks(K) * B8_BLOCK, all = (T + 63) / 64;
-  const long long t256 = (long long)((N + 255) / 256) * ((kp + 255) / 256);
-  w.big = t256 >= 32;
-  const int b = w.big ? 256 : 128;
-  w.tiles_n = (N + b - 1) / b;
-  w.tiles_k = (kp + b - 1) / b;
-  const long long tiles = (long long)w.tiles_n * w.tiles_k, want = w.big ? 256 : 512;
-  // at least 2 steps per split: a split costs a round trip of its partial sums through memory
-  long long splits = want / tiles;
-  if (splits > all / 2) splits = all / 2;
-  if (splits < 1) splits = 1;
-  w.steps = (int)((all + splits - 1) / splits);
-  w.splits = (all + w.steps - 1) / w.steps;
-  return w;
+  W8Plan best{};
+  double best_us = 0;
+  for (int big = 0; big < 2; ++big) {
+    const int b = big ? 256 : 128, tn = (N + b - 1) / b, tk = (kp + b - 1) / b;
+    const long long tiles = (long long)tn * tk;
+    for (int want : tries) {
+      if (want > 1 && (want > all || tiles * (want - 1) > 1024)) break;
+      const int steps = (all + want - 1) / want, splits = (all + steps - 1) / steps;
+      const long long per_cu = (tiles * splits + 255) / 256;
+      const double step = big ? 1.67 * per_cu : per_cu == 1 ? 0.8 : 1.17 * ((per_cu + 1) / 2);
+      const double us = 4 + steps * step + (splits > 1 ? 4 + 8e-6 / 4 * splits * N * K : 0);
+      if (best.steps == 0 || us < best_us) {
+        best_us = us;
+        best = W8Plan{big != 0, tn, tk, splits, steps};
+      }
+    }
+  }
+  return best;
 }
 
 extern "C" size_t sdamd_linear8_weight_grad_ws_bytes(int T, int N, int K) {
