@@ -1,8 +1,9 @@
 // 8-bit blocks (blocks8.h): quantise, dequantise, and GeGLU (diffusion.py:128-130) with its pre-activation kept in them.
-// All of it is bound by HBM: one pass, 16-byte loads, nothing read twice.
+// All of it is bound by HBM: one pass, 16-byte loads, nothing read twice.  (Sizes are limited by a launch's 2^32 threads.)
 #include "blocks8.h"
 
-// ---- rows -> blocks.  q [rows][KB*128], scale [rows][SP]; 16 lanes hold a block, a workgroup takes 16 * UN blocks.
+// ---- rows -> blocks.  q [rows][KB*128], scale [rows][SP]; 16 lanes hold a block, a workgroup takes 16 * UN blocks, all of
+// them requested before the first is used.  36864 x 1280 bf16: 24.9 us = 5.7 TB/s with UN = 2 (1: 31.1, 4: 26.3).
 template <typename T, int UN>
 __global__ __launch_bounds__(256) void quant8_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
                                                      unsigned char* __restrict__ scale, unsigned nblk, int KB, int K,
@@ -91,6 +92,7 @@ __global__ __launch_bounds__(256) void dequant8_kernel(const unsigned char* __re
 }
 
 // ---- GeGLU that keeps its input in 8 bits: h [rows][2F] -> out [rows][F] = value * gelu(gate), and h's blocks.
+// 65536 x 1280 bf16: 119 us = 5.6 TB/s.
 // F % 128 == 0: the 16 lanes that hold a value block hold the gate block of the same columns too, so h is read once.
 template <typename T>
 __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned char* __restrict__ q,
@@ -144,7 +146,7 @@ __device__ __forceinline__ void gelu_slope(float x, float& gelu, float& slope) {
   slope = __builtin_fmaf(x * 0.39894228040143267794f, e, cdf);
 }
 
-// ---- GeGLU backward: dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
+// ---- GeGLU backward (65536 x 1280 bf16 from e4m3: 130 us = 5.2 TB/s): dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
 // (TH = unsigned char)
 template <typename TD, typename TH, typename TO>
 __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restrict__ dout, const TH* __restrict__ h,
@@ -197,7 +199,7 @@ extern "C" int sdamd_quant8(const void* x, void* q, unsigned char* scale, long l
   SD_CHECK(is_val(dtype) && is_fmt(fmt), "quant8: unsupported dtypes in=%d out=%d", dtype, fmt);
   SD_CHECK(rows > 0 && K > 0 && K <= (1 << 30) && ldx >= 0, "quant8: bad shape rows=%lld K=%d", rows, K);
   const int KB = b8_kblocks(K);
-  SD_CHECK(rows * (long long)KB < (1ll << 31), "quant8: too large, rows=%lld K=%d", rows, K);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)KB < (1ll << 29), "quant8: too large, rows=%lld K=%d", rows, K);
   const unsigned nblk = (unsigned)(rows * KB);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == SDAMD_BF16)
@@ -226,7 +228,7 @@ extern "C" int sdamd_dequant8(const void* q, const unsigned char* scale, void* o
   SD_CHECK(is_val(out_dtype) && is_fmt(fmt), "dequant8: unsupported dtypes in=%d out=%d", fmt, out_dtype);
   SD_CHECK(rows > 0 && K > 0 && K <= (1 << 30) && (block_rows == 1 || block_rows == B8_BLOCK), "dequant8: bad shape rows=%lld K=%d block_rows=%d", rows, K, block_rows);
   const int KB = b8_kblocks(K);
-  SD_CHECK(rows * (long long)KB < (1ll << 31), "dequant8: too large, rows=%lld K=%d", rows, K);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)KB < (1ll << 28), "dequant8: too large, rows=%lld K=%d", rows, K);
   const unsigned nblk = (unsigned)(rows * KB);
   const int shift = block_rows == 1 ? 0 : 7, SP = b8_scale_stride(K);
   hipStream_t st = (hipStream_t)stream;
@@ -255,7 +257,7 @@ static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned ch
 extern "C" int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt, void* stream) {
   SD_CHECK(is_val(dtype) && is_fmt(fmt), "geglu_train: unsupported dtypes h=%d kept=%d", dtype, fmt);
   SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_train: bad shape rows=%lld F=%d", rows, F);
-  SD_CHECK(rows * (long long)((F + 7) / 8) < (1ll << 31), "geglu_train: too large, rows=%lld F=%d", rows, F);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)((F + 7) / 8) < (1ll << 31), "geglu_train: too large, rows=%lld F=%d", rows, F);
   if (dtype == SDAMD_BF16) geglu_train_launch<bf16_t>((const bf16_t*)h, (bf16_t*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
   else geglu_train_launch<float>((const float*)h, (float*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
   SD_LAUNCH_CHECK("geglu_train");
@@ -269,7 +271,7 @@ extern "C" int sdamd_geglu_backward(const void* dout, const void* h, const unsig
   SD_CHECK(!is_fmt(h_dtype) || h_scale, "geglu_backward: 8-bit h without its scales");
   SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_backward: bad shape rows=%lld F=%d", rows, F);
   const int VR = (F + 7) / 8;
-  SD_CHECK(rows * (long long)VR < (1ll << 31), "geglu_backward: too large, rows=%lld F=%d", rows, F);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)VR < (1ll << 31), "geglu_backward: too large, rows=%lld F=%d", rows, F);
   const unsigned nvec = (unsigned)(rows * VR);
   hipStream_t st = (hipStream_t)stream;
   const int SP = b8_scale_stride(2 * F), ldq = b8_kblocks(2 * F) * B8_BLOCK;

@@ -319,6 +319,7 @@ extern "C" int sdamd_layernorm_backward(const void* dy, const void* x, const uns
            x_dtype >= SDAMD_F32 && x_dtype <= SDAMD_E5M2, "layernorm_backward: unsupported dtypes dy=%d x=%d dx=%d", dy_dtype, x_dtype, dx_dtype);
   SD_CHECK(x_dtype < SDAMD_E4M3 || x_scale, "layernorm_backward: 8-bit x without its scales");
   SD_CHECK(rows > 0 && C > 0 && C <= LNT_MAX_C, "layernorm_backward: unsupported shape rows=%d C=%d (C <= %d)", rows, C, LNT_MAX_C);
+  SD_CHECK(rows <= (1 << 28), "layernorm_backward: too many rows, %d", rows);
   const size_t need = sdamd_layernorm_backward_ws_bytes(rows, C);
   SD_CHECK(need == 0 || (ws && ws_bytes >= need), "layernorm_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
   hipStream_t st = (hipStream_t)stream;

@@ -267,6 +267,7 @@ __global__ __launch_bounds__(256) void wgrad8_reduce(const float* __restrict__ p
 // ---------------------------------------------------------------------------------------------
 // host entry points
 // ---------------------------------------------------------------------------------------------
+constexpr int W8_MAX_WIDTH = 1 << 24;            // (offsets within 64 rows are held in 32 bits)
 struct W8Plan { bool big; int tiles_n, tiles_k, splits, steps; };
 // Tile size and number of splits by the least estimated time, in us, from what the kernels measured: a step of 64 tokens
 // takes 1.67 with one 256 x 256 workgroup on a CU, 0.8 with one of 128 x 128 and 1.17 with two; a split result costs its
@@ -297,7 +298,7 @@ static W8Plan w8_plan(int T, int N, int K) {
 }
 
 extern "C" size_t sdamd_linear8_weight_grad_ws_bytes(int T, int N, int K) {
-  if (T <= 0 || N <= 0 || K <= 0) return 0;
+  if (T <= 0 || N <= 0 || K <= 0 || N > W8_MAX_WIDTH || K > W8_MAX_WIDTH) return 0;
   const W8Plan w = w8_plan(T, N, K);
   return w.splits > 1 ? (size_t)w.splits * ((size_t)N * K + N) * sizeof(float) : 0;
 }
@@ -316,9 +317,11 @@ static int w8_launch(const W8Args& p, int splits, hipStream_t st) {
 extern "C" int sdamd_linear8_weight_grad(const void* dy, const void* x8, const unsigned char* x8_scale, float* dw, float* db, void* ws, size_t ws_bytes,
                                          int T, int N, int K, int fmt, void* stream) {
   SD_CHECK(fmt == SDAMD_E4M3 || fmt == SDAMD_E5M2, "linear8_weight_grad: unsupported dtype %d", fmt);
-  SD_CHECK(T > 0 && N > 0 && K > 0 && N <= (1 << 30) && K <= (1 << 30) && T <= (1 << 30), "linear8_weight_grad: bad shape T=%d N=%d K=%d", T, N, K);
+  SD_CHECK(T > 0 && N > 0 && K > 0 && N <= W8_MAX_WIDTH && K <= W8_MAX_WIDTH && T <= (1 << 30),
+           "linear8_weight_grad: bad shape T=%d N=%d K=%d (N, K <= %d)", T, N, K, W8_MAX_WIDTH);
+  SD_CHECK(((uintptr_t)x8 & 15) == 0 && ((uintptr_t)x8_scale & 3) == 0, "linear8_weight_grad: blocks have to be 16-byte aligned, their scales 4-byte aligned");
   const W8Plan w = w8_plan(T, N, K);
-  SD_CHECK((long long)w.tiles_n * w.tiles_k < (1ll << 31), "linear8_weight_grad: too large, N=%d K=%d", N, K);
+  SD_CHECK((long long)w.tiles_n * w.tiles_k < (1ll << 23), "linear8_weight_grad: too large, N=%d K=%d", N, K);
   const size_t need = sdamd_linear8_weight_grad_ws_bytes(T, N, K), nk = (size_t)N * K;
   SD_CHECK(need == 0 || (ws && ws_bytes >= need), "linear8_weight_grad: workspace of %zu bytes, %zu needed", ws_bytes, need);
   float* part = (float*)ws;

@@ -775,6 +775,12 @@ def _dev8(name, first, *others):
     return first.device
 
 
+def _fits(name, *sizes):
+    """Sizes that cross the C boundary as ints (ctypes would cut them silently)."""
+    if max(sizes) > 0x7fffffff:
+        raise _lib.SdamdError(f"{name}: size {max(sizes)} is too large")
+
+
 def _vec_f32(name, what, t, n):
     _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, "%s: %s has to be %d contiguous float32 values", name, what, n)
 
@@ -784,7 +790,9 @@ class Blocks8:
     2^(byte - 127) per 128 columns of a row (``block_rows`` = 1: activations, checkpoints) or per 128 x 128 block
     (``block_rows`` = 128: weights, e4m3), ``scale`` [rows / block_rows, K / 128 up to 4] uint8.  ``shape`` is the shape
     of the values it stands for.  Made by ``quantize8`` / ``quantize8_weight`` or from stored bytes; columns of ``q``
-    past K have to be zero bytes.  Of an infinity e4m3 keeps NaN, e5m2 keeps it; NaN stays NaN; neither counts for the scale."""
+    past K have to be zero bytes.  Of an infinity e4m3 keeps NaN, e5m2 keeps it; NaN stays NaN; neither counts for the scale.
+    Scale bytes from elsewhere may be any, 255 standing for NaN; values beyond float32's range are infinities wherever they
+    are taken as bfloat16 or float32 (``dequantize``, float32 results, gradients)."""
 
     __slots__ = ("q", "scale", "shape", "block_rows")
 
@@ -849,6 +857,7 @@ def quantize8(x, dtype=torch.float8_e4m3fn):
     if not (x.dim() >= 1 and x.shape[-1] > 0 and (x.is_contiguous() or (x.dim() == 2 and x.stride(1) == 1))):
         raise _lib.SdamdError("quantize8: shape %s, strides %s" % (tuple(x.shape), tuple(x.stride())))
     K = x.shape[-1]
+    _fits("quantize8", K)
     out = _blocks8_empty(x.shape, dtype, dev)
     rows = out.q.shape[0]
     if rows:
@@ -866,6 +875,7 @@ def quantize8_weight(w):
     if not (w.dim() == 2 and w.shape[0] > 0 and w.shape[1] > 0):
         raise _lib.SdamdError("quantize8_weight: shape %s" % (tuple(w.shape),))
     N, K = w.shape
+    _fits("quantize8_weight", N, K)
     kb = -(-K // BLOCK8)
     q = torch.empty((N, kb * BLOCK8), dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty((-(-N // BLOCK8), -(-kb // 4) * 4), dtype=torch.uint8, device=dev)
@@ -878,8 +888,8 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     """act(x @ w^T + bias + residual) -> [..., N] with both operands in 8-bit blocks: ``w`` from ``quantize8_weight``;
     ``x`` Blocks8, or float32 / bfloat16 [..., K], then quantised to ``fmt`` on the way (``gemm``'s act: none, quick-gelu,
     silu).  ``out_dtype`` (default: the residual's, else x's, else bfloat16): a bfloat16 result takes the matrix core's
-    scaled 8-bit products, whose internal sums are good to 1e-5 of the result; a float32 result is summed in float32 from
-    exact products at half that rate."""
+    scaled 8-bit products, which it aligns 2^-20 below the largest of each 128 (1e-5 of the result, a hundredth of its own
+    rounding); a float32 result is summed in float32 from exact products at half that rate."""
     is8 = isinstance(x, Blocks8)
     if not (isinstance(w, Blocks8) and w.block_rows == BLOCK8):
         raise _lib.SdamdError("linear8: w has to come from quantize8_weight")
@@ -897,6 +907,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
         raise _lib.SdamdError("linear8: unsupported activation %s" % (act,))
     shape = tuple(x.shape[:-1]) + (N,)
     M = math.prod(shape[:-1])
+    _fits("linear8", M, N, K)
     if bias is not None:
         _vec_f32("linear8", "bias", bias, N)
     if residual is not None:
@@ -937,6 +948,7 @@ def linear8_weight_grad(dy, x8, bias=True):
     if not (dy.dim() >= 1 and dy.is_contiguous() and tuple(dy.shape[:-1]) == x8.shape[:-1] and dy.shape[-1] > 0):
         raise _lib.SdamdError("linear8_weight_grad: dy %s has to be contiguous beside x8 %s" % (tuple(dy.shape), x8.shape))
     N, K, T = dy.shape[-1], x8.shape[-1], x8.q.shape[0]
+    _fits("linear8_weight_grad", N, K, T)
     if T == 0:
         return torch.zeros((N, K), dtype=torch.float32, device=dev), torch.zeros(N, dtype=torch.float32, device=dev) if bias else None
     dw = torch.empty((N, K), dtype=torch.float32, device=dev)
@@ -961,15 +973,16 @@ def layernorm_train(x, gamma, beta, eps=1e-5, out_dtype=None):
     _vec_f32("layernorm_train", "beta", beta, C)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     rows = x.numel() // C
+    _fits("layernorm_train", rows, C)
     if out_dtype in _FMT8:
         y = _blocks8_empty(x.shape, out_dtype, dev)
         yp, sp, out_code, size = y.q, y.scale, _code8(out_dtype), 1
     else:
         out_code = _code(out_dtype)
-        y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+        y = torch.empty_like(x) if out_dtype == x.dtype else torch.empty(x.shape, dtype=out_dtype, device=dev)
         yp, sp, size = y, None, y.element_size()
     mean = torch.empty(rows, dtype=torch.float32, device=dev)
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    rstd = torch.empty_like(mean)
     if rows:
         _run8(dev, "sdamd_layernorm_train", (_p(x), _p(yp), _p(sp), _p(gamma), _p(beta), _p(mean), _p(rstd), rows, C, float(eps), code, out_code),
               lambda: ("layernorm_train", x.numel() * (x.element_size() + size), f"rows{rows} C{C}", 0.0))
@@ -989,6 +1002,7 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
         raise _lib.SdamdError("layernorm_backward: dy %s has to be contiguous beside x %s" % (tuple(dy.shape), tuple(x.shape)))
     C = dy.shape[-1]
     rows = dy.numel() // C
+    _fits("layernorm_backward", rows, C)
     _vec_f32("layernorm_backward", "gamma", gamma, C)
     _vec_f32("layernorm_backward", "mean", mean, rows)
     _vec_f32("layernorm_backward", "rstd", rstd, rows)
@@ -998,11 +1012,11 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
     if residual is not None:
         if not (residual.dtype == out_dtype and residual.is_contiguous() and residual.shape == dy.shape):
             raise _lib.SdamdError("layernorm_backward: residual %s %s has to be a contiguous %s %s" % (residual.dtype, tuple(residual.shape), out_dtype, tuple(dy.shape)))
-    dx = torch.empty(dy.shape, dtype=out_dtype, device=dev)
+    dx = torch.empty_like(dy) if out_dtype == dy.dtype else torch.empty(dy.shape, dtype=out_dtype, device=dev)
     if rows == 0:
         return dx, torch.zeros(C, dtype=torch.float32, device=dev), torch.zeros(C, dtype=torch.float32, device=dev)
     dgamma = torch.empty(C, dtype=torch.float32, device=dev)
-    dbeta = torch.empty(C, dtype=torch.float32, device=dev)
+    dbeta = torch.empty_like(dgamma)
     need = _lib.lib().sdamd_layernorm_backward_ws_bytes(rows, C)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _run8(dev, "sdamd_layernorm_backward", (_p(dy), _p(x.q if is8 else x), _p(x.scale if is8 else None), _p(gamma), _p(mean), _p(rstd),
@@ -1020,6 +1034,7 @@ def geglu_train(h, dtype=torch.float8_e4m3fn):
     if not (h.dim() >= 1 and h.is_contiguous() and h.shape[-1] > 0 and h.shape[-1] % 2 == 0):
         raise _lib.SdamdError("geglu_train: shape %s, strides %s" % (tuple(h.shape), tuple(h.stride())))
     Fh = h.shape[-1] // 2
+    _fits("geglu_train", 2 * Fh)
     out = torch.empty(h.shape[:-1] + (Fh,), dtype=h.dtype, device=dev)
     kept = _blocks8_empty(h.shape, dtype, dev)
     rows = kept.q.shape[0]
@@ -1042,7 +1057,8 @@ def geglu_backward(dout, h, out_dtype=None):
     dcode, hcode, ocode = _code(dout.dtype), _code8(h.dtype) if is8 else _code(h.dtype), _code(out_dtype)
     Fh = dout.shape[-1]
     rows = dout.numel() // Fh
-    dh = torch.empty(tuple(h.shape), dtype=out_dtype, device=dev)
+    _fits("geglu_backward", 2 * Fh)
+    dh = torch.empty_like(h) if not is8 and h.dtype == out_dtype else torch.empty(h.shape, dtype=out_dtype, device=dev)
     if rows:
         _run8(dev, "sdamd_geglu_backward", (_p(dout), _p(h.q if is8 else h), _p(h.scale if is8 else None), _p(dh), rows, Fh, dcode, hcode, ocode),
               lambda: ("geglu_backward", dh.numel() * (dh.element_size() + (1 if is8 else h.element_size()) + dout.element_size() / 2),

@@ -281,6 +281,55 @@ def test_linear8_shapes_out_and_refusals():
             call()
 
 
+def test_scale_bytes_of_any_value():
+    """Blocks made elsewhere may carry any scale byte: 2^-127 (0) to 2^127 (254), and 255, which stands for NaN."""
+    M, K, N = 40, 256, 130
+    x = ops.quantize8((rnd(1, (M, K)).sign() * 256).to(DEV))
+    w = ops.quantize8_weight(rnd(2, (N, K)).to(DEV))
+    bytes_ = [0, 1, 60, 127, 200, 254, 255, 130]
+    for r in range(M):
+        x.scale[r, :2] = bytes_[r % len(bytes_)]
+    w.scale[:, :2] = 70                                  # 2^-57
+    vals = np64(x.q) * np.repeat(2.0 ** (x.scale[:, :2].cpu().numpy().astype(np.float64) - 127), 128, 1)
+    nan = x.scale[:, 0].cpu().numpy() == 255
+    wv = np64(w.q) * 2.0 ** -57
+    want = vals @ wv.T
+    top = np.finfo(np.float32).max
+    # 2^127 * 256 is beyond float32 (and bfloat16, of the same range): where values are taken in those types, such a one is an
+    # infinity, like in any conversion.  The bfloat16 form of the product takes the bytes themselves.
+    with np.errstate(over="ignore"):
+        held = vals.astype(np.float32).astype(np.float64)
+    for out in (BF16, F32):
+        for rows in (slice(0, 8), slice(0, M)):
+            part = ops.Blocks8(x.q[rows].contiguous(), x.scale[rows].contiguous(), (len(range(*rows.indices(M))), K))
+            got = np64(ops.linear8(part, w, out_dtype=out))
+            assert np.isnan(got[nan[rows]]).all()
+            ok = ~nan[rows] & (np.isfinite(held[rows]).all(1) if out == F32 else True)
+            assert not np.isfinite(got[~ok]).any() and (np.abs(want[rows][ok]) < top).all()
+            # scale byte 0 puts results at 2^-127 2^8 2^-57 2^8 sqrt(256) = 2^-164, below everything an f32 or bf16 holds: such
+            # a result is off by itself, less than the smallest normal number 2^-126
+            close(got[ok], want[rows][ok], 2.0 ** -126 + linear_tol(vals[rows][ok], wv, np.abs(vals[rows][ok]) @ np.abs(wv).T, out, want[rows][ok], 0))
+    assert np.isnan(np64(x.dequantize(F32))[nan]).all() and np.array_equal(np64(x.dequantize(F32))[~nan], held[~nan])
+    dy = torch.zeros(M, 24, dtype=BF16)
+    dy[4:6] = 2.0 ** -60                                 # scales 2^73 and 2^127
+    dw, _ = ops.linear8_weight_grad(dy[4:6].contiguous().to(DEV), ops.Blocks8(x.q[4:6].contiguous(), x.scale[4:6].contiguous(), (2, K)))
+    assert np.isinf(held[5]).all() and np.array_equal(np64(dw), np64(dy[4:6]).T @ held[4:6])
+    dw, _ = ops.linear8_weight_grad(dy[6:7].contiguous().to(DEV), ops.Blocks8(x.q[6:7].contiguous(), x.scale[6:7].contiguous(), (1, K)))
+    assert dw.isnan().all()
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_linear8_under_plan_samples(out):
+    """Deterministic plans: a sample's rows give the same bits alone and in any batch."""
+    S, R, K, N = 24, 77, 320, 640
+    x, w = rnd(3, (S * R, K)).to(DEV), ops.quantize8_weight(rnd(4, (N, K)).to(DEV))
+    with ops.plan_samples(1):
+        alone = ops.linear8(x[5 * R:6 * R], w, out_dtype=out)
+    with ops.plan_samples(S):
+        batch = ops.linear8(x, w, out_dtype=out)
+    assert torch.equal(batch[5 * R:6 * R], alone)
+
+
 # ------------------------------------------------------------------ weight gradient
 @pytest.mark.parametrize("T,N,K", [(1, 1, 1), (3, 8, 130), (64, 16, 128), (77, 40, 300), (1003, 333, 215), (130, 1280, 320),
                                    (4100, 264, 257), (700, 2100, 1100), (640, 2056, 1024)])

@@ -30,6 +30,15 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 1, 0), "without their scales")
     refused(L.sdamd_linear8(P, 0, P, P, P, 0, 0, 9000, 4096, 4096, 0, 1, 2, 1, 0), "quantised first")
     assert L.sdamd_linear8_quantises(1, 1280, 320, 1) == 1 and L.sdamd_linear8_quantises(9000, 4096, 4096, 1) == 0 and L.sdamd_linear8_quantises(0, 1, 1, 0) == 0
+    refused(L.sdamd_linear8(P, P, P, P, P, 0, 0, 4, 4, (1 << 24) + 1, 0, 2, 2, 1, 0), "bad shape")
+    refused(L.sdamd_linear8(P + 8, P, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 1, 0), "aligned")
+    refused(L.sdamd_linear8(P, P + 2, P, P, P, 0, 0, 4, 4, 4, 0, 2, 2, 1, 0), "aligned")
+    refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, (1 << 24) + 1, 4, 2, 0), "bad shape")
+    refused(L.sdamd_linear8_weight_grad(P, P + 4, P, P, P, 0, 0, 4, 4, 4, 2, 0), "aligned")
+    refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 1 << 24, 768, 1e-5, 0, 0, 0), "too many rows")
+    refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, 1 << 30, 1 << 29, 8, 0, 0, 0, 0), "too many rows")
+    refused(L.sdamd_geglu_train(P, P, P, P, 1 << 40, 64, 0, 2, 0), "too large")
+    refused(L.sdamd_geglu_backward(P, P, 0, P, 1 << 40, 64, 0, 0, 0, 0), "too large")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 0, 4, 4, 2, 0), "bad shape")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, 4, 4, 1, 0), "unsupported dtype")
     need = L.sdamd_linear8_weight_grad_ws_bytes(65536, 320, 320)
@@ -70,6 +79,13 @@ def test_python_refuses_the_cpu_and_bad_blocks():
             ops.Blocks8(*args)
     with pytest.raises(TypeError):
         ops.Blocks8(q.view(torch.int8), s, (4, 200))
+
+
+def test_sizes_are_not_cut_at_the_boundary():
+    """ctypes would pass 2^32 + 5 as 5."""
+    ops._fits("x", 1, 0x7fffffff)
+    with pytest.raises(_lib.SdamdError, match="too large"):
+        ops._fits("x", 5, (1 << 32) + 5)
 
 
 def test_workspaces_cover_their_plans():
