@@ -5,9 +5,9 @@
 //   a = dy gamma,  dx = rstd (a - sum a / C - xh sum(a xh) / C) (+ residual)
 //   dgamma = sum_rows dy xh,  dbeta = sum_rows dy
 //
-// G lanes share a row and keep it in registers, NV vectors of 8 values per lane: 256 / G rows per workgroup and no lane idle
-// at the widths of the UNet (320 = 8 lanes x 5, 640 = 16 x 5, 1280 = 32 x 5).  Rows are read once per pass; both passes
-// are bound by HBM.  The variance is taken from the centred values, so a large mean costs no digits.
+// G lanes share a row and keep it in registers, NV vectors of 8 values per lane.  Rows are read once per pass; both passes
+// are bound by HBM where there are enough rows.  The variance is taken from the centred values, so a large mean costs no
+// digits.
 #pragma once
 #include "blocks8.h"
 
@@ -27,15 +27,3 @@ template <int G> __device__ __forceinline__ float group_sum(float v, float* red)
   }
   return v;
 }
-
-// lanes per row and vectors per lane for a row of nvec vectors: the fewest lanes that hold it in at most 6 vectors each
-// (more rows per wave and fewer shuffles per reduction), never more than 256
-#define LNT_PICK(nvec, CASE)                                                                                      \
-  do {                                                                                                            \
-    const int nv_ = (nvec);                                                                                       \
-    if (nv_ <= 16) { CASE(8, 2); } else if (nv_ <= 32) { CASE(8, 4); } else if (nv_ <= 40) { CASE(8, 5); }         \
-    else if (nv_ <= 48) { CASE(8, 6); } else if (nv_ <= 64) { CASE(16, 4); } else if (nv_ <= 80) { CASE(16, 5); }  \
-    else if (nv_ <= 96) { CASE(16, 6); } else if (nv_ <= 128) { CASE(32, 4); } else if (nv_ <= 160) { CASE(32, 5); } \
-    else if (nv_ <= 192) { CASE(32, 6); } else if (nv_ <= 256) { CASE(64, 4); } else if (nv_ <= 384) { CASE(64, 6); } \
-    else if (nv_ <= 512) { CASE(256, 2); } else if (nv_ <= 1024) { CASE(256, 4); } else { CASE(256, 6); }          \
-  } while (0)
