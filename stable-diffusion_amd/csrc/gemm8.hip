@@ -442,12 +442,14 @@ static bool g8_few_rows(int rows, int N, bool exact) {
   const int M = plan_rows(rows);
   return (M <= 64 || g8_tiles(M, N, 128) < (exact ? 64 : 32)) && (rows + 63) / 64 <= 65535;
 }
-// That kernel can quantise rows on its way.  Every workgroup then repeats the work for its rows, so it does where that is
-// cheaper than a launch of its own: up to G8_RAW_WORK values over all workgroups.
-constexpr long long G8_RAW_WORK = 1ll << 24;
+// That kernel can quantise rows on its way.  A wave then quantises its blocks of K for all the workgroup's 16-row tiles, which
+// saves the launch and the buffers of quantising first (9 us of host work a call) and costs more on the GPU the more of
+// them there are: 1 x 320 -> 1280: 3.4 us, first quantised 4.7; 16 x 1280 -> 1280: 5.7 and 6.3; 154 x 768 -> 640 (4 a wave): 9.5
+// and 7.7; 64 x 1280 -> 640 (8): 13.7 and 9.1; 64 x 5120 -> 320 (20): 42 and 18.  So up to 4 a wave.
 extern "C" int sdamd_linear8_quantises(int M, int N, int K, int out_dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return g8_few_rows(M, N, out_dtype == SDAMD_F32) && (long long)((N + 15) / 16) * M <= G8_RAW_WORK / K;
+  const int tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  return g8_few_rows(M, N, out_dtype == SDAMD_F32) && (b8_kblocks(K) + 7) / 8 * tiles <= 4;
 }
 
 template <int BM, int BN, int WGM, int WGN, int PLACES, int FMT, bool EXACT, typename TO>
