@@ -15,7 +15,6 @@
 #define SDAMD_E5M2 3
 
 constexpr int B8_BLOCK = 128;      // values that share a scale (weights: 128 rows x 128 columns)
-constexpr int B8_LANES = 16;       // lanes that hold a row's block, 8 values each
 
 static inline int b8_kblocks(int K) { return (K + B8_BLOCK - 1) / B8_BLOCK; }
 static inline int b8_scale_stride(int K) { return (b8_kblocks(K) + 3) / 4 * 4; }   // bytes of scale per row: whole 32-bit words
@@ -75,11 +74,16 @@ __device__ __forceinline__ void b8_unpack8(u32x2_t q, int e, int fmt, float (&v)
     v[4 * h] = lo[0] * s; v[4 * h + 1] = lo[1] * s; v[4 * h + 2] = hi[0] * s; v[4 * h + 3] = hi[1] * s;
   }
 }
-// largest magnitude over the 16 lanes that hold a block
+// largest magnitude over the 16 lanes that hold a block: rotations within the 16, in the vector unit (data-parallel
+// primitives; __shfl would go through LDS four times)
+template <int N> __device__ __forceinline__ unsigned b8_rotate16(unsigned m) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x120 + N, 0xf, 0xf, true);
+}
 __device__ __forceinline__ unsigned b8_max16(unsigned m) {
-#pragma unroll
-  for (int o = B8_LANES / 2; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-  return m;
+  m = max(m, b8_rotate16<8>(m));
+  m = max(m, b8_rotate16<4>(m));
+  m = max(m, b8_rotate16<2>(m));
+  return max(m, b8_rotate16<1>(m));
 }
 __device__ __forceinline__ unsigned b8_mag8(const float (&v)[8]) {
   unsigned m = 0;

@@ -344,86 +344,119 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// 16 columns and up to 16 * MT rows per workgroup; its 8 waves share out the blocks of K and read them straight into
-// registers (every weight byte is used once: LDS would only delay it), then join their sums in a fixed order in LDS.
-// XRAW: A is the f32 / bf16 rows themselves, quantised on the way in (a block of a row lies in the four lanes 16 apart).
+// 16 columns and up to 16 * MT rows per workgroup; its 16 waves (8 where they have 64 rows) share out the blocks of K and
+// join their sums in a fixed order at the end.  Each wave has an LDS region of its own for a step's rows, so there is no barrier in the loop: memory is
+// read in whole 128-byte rows by neighbouring lanes (a fragment load straight from memory, 16 rows x 64 bytes, takes the
+// address unit three times as long: 256 x 5120 -> 1280 took 27 us).
+// XRAW: A is the f32 / bf16 rows themselves; 16 lanes take a row's block, quantise it and leave the bytes in that region.
+template <int MT> constexpr int g8_rows_waves() { return MT == 4 ? 8 : 16; }
+template <int MT> constexpr int g8_rows_lds() { return g8_rows_waves<MT>() * (MT + 1) * 16 * 128; }     // (the sums take less)
 template <int MT, int FMT, bool EXACT, typename TO, typename TX>
-__global__ __launch_bounds__(512) void gemm8_rows_kernel(G8Args p) {
+__global__ __launch_bounds__(64 * g8_rows_waves<MT>()) void gemm8_rows_kernel(G8Args p) {
   constexpr bool XRAW = sizeof(TX) != 1;
+  constexpr int NW = g8_rows_waves<MT>();
   constexpr int LD = 20;                                   // floats per row of the exchange: 16 columns, 16-byte aligned
-  __shared__ __attribute__((aligned(16))) float ex[8][MT * 16][LD];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];   // per wave [MT * 16 + 16][128] activations, weights; then [NW][MT * 16][LD] sums
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-  const unsigned char* wr = p.W + (size_t)min(n0 + r16, p.N - 1) * p.KB * B8_BLOCK + g * 32;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT, ldb = p.KB * B8_BLOCK;
+  char* mine = smem + wave * (MT + 1) * 16 * 128;
+  const unsigned char *baseA = (const unsigned char*)p.A + (size_t)m0 * ldb, *baseW = p.W + (size_t)n0 * ldb;
   const unsigned char* sw = p.Ws + (size_t)(n0 / B8_BLOCK) * p.SP;
+  // offsets of the rows a lane fetches: 8 rows an instruction, the 16-byte chunks of a row permuted by (row >> 1) & 7
+  unsigned off_a[XRAW ? 1 : 2 * MT], off_w[2];
+#pragma unroll
+  for (int i = 0; i < 2 * MT + 2; ++i) {
+    const int row = (i < 2 * MT ? i : i - 2 * MT) * 8 + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
+    if (i >= 2 * MT) off_w[i - 2 * MT] = (unsigned)min(row, p.N - 1 - n0) * (unsigned)ldb + ch * 16;
+    else if (!XRAW) off_a[XRAW ? 0 : i] = (unsigned)min(row, p.M - 1 - m0) * (unsigned)ldb + ch * 16;
+  }
+  const unsigned in_row = r16 * 128 + ((g ^ (r16 >> 1)) << 4);
+  auto frag = [&](int tile) {
+    const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(mine + tile * 2048 + in_row), hi = *reinterpret_cast<const u32x4_t*>(mine + tile * 2048 + (in_row ^ 64u));
+    return (i32x8_t){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
   f32x4_t acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < p.KB; kb += 8) {
-    const u32x4_t* wp = reinterpret_cast<const u32x4_t*>(wr + (size_t)kb * B8_BLOCK);
-    const u32x4_t w0 = wp[0], w1 = wp[1];
-    const int bw = sw[kb];
-    i32x8_t a[MT];
+  const int per = (p.KB + NW - 1) / NW, k_end = min(p.KB, (wave + 1) * per);
+  unsigned word_a[MT], word_w = 0;                         // four blocks' scales
+  for (int kb = wave * per; kb < k_end; ++kb) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // (the last step's fragments are read)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma16(baseW + (size_t)kb * B8_BLOCK, off_w[i], mine + (2 * MT + i) * 1024);
     int ba[MT];
     if constexpr (!XRAW) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const size_t m = min(m0 + i * 16 + r16, p.M - 1);
-        const u32x4_t* ap = reinterpret_cast<const u32x4_t*>((const unsigned char*)p.A + (m * p.KB + kb) * B8_BLOCK + g * 32);
-        const u32x4_t a0 = ap[0], a1 = ap[1];
-        ba[i] = p.As[m * p.SP + kb];
-        a[i] = (i32x8_t){(int)a0[0], (int)a0[1], (int)a0[2], (int)a0[3], (int)a1[0], (int)a1[1], (int)a1[2], (int)a1[3]};
-      }
-    } else {
+      for (int i = 0; i < 2 * MT; ++i) dma16(baseA + (size_t)kb * B8_BLOCK, off_a[XRAW ? 0 : i], mine + i * 1024);
+    }
+    if ((kb & 3) == 0 || kb == wave * per) {
+      word_w = *reinterpret_cast<const unsigned*>(sw + (kb & ~3));
+      if constexpr (!XRAW) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const size_t m = min(m0 + i * 16 + r16, p.M - 1);
-        const TX* xr = (const TX*)p.A + m * p.K;
-        Raw8<TX> raw[4];
-        float v[4][8];
-        unsigned mag = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) raw[q] = raw8_load(xr, kb * B8_BLOCK + g * 32 + q * 8, p.K);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          raw8_get(raw[q], kb * B8_BLOCK + g * 32 + q * 8, p.K, v[q]);
-          mag = max(mag, b8_mag8(v[q]));
-        }
-        mag = max(mag, (unsigned)__shfl_xor((int)mag, 16, 64));
-        mag = max(mag, (unsigned)__shfl_xor((int)mag, 32, 64));
-        ba[i] = b8_exponent_of(mag, FMT);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const u32x2_t t = b8_pack8(v[q], ba[i], FMT);
-          a[i][2 * q] = (int)t[0];
-          a[i][2 * q + 1] = (int)t[1];
-        }
+        for (int i = 0; i < MT; ++i) word_a[i] = *reinterpret_cast<const unsigned*>(p.As + (size_t)min(m0 + i * 16 + r16, p.M - 1) * p.SP + (kb & ~3));
       }
     }
-    const i32x8_t w = {(int)w0[0], (int)w0[1], (int)w0[2], (int)w0[3], (int)w1[0], (int)w1[1], (int)w1[2], (int)w1[3]};
-    if constexpr (!EXACT) {
+    if constexpr (XRAW) {
+      const int c = kb * B8_BLOCK + r16 * 8;
+      Raw8<TX> raw[4], next[4];
+      auto fetch = [&](int i, Raw8<TX> (&to)[4]) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = mfma8<FMT>(a[i], w, acc[i], ba[i], bw);
-    } else {
-      const Bf4 wb = to_bf16<SDAMD_E4M3>(w, b8_scale(bw));
+        for (int q = 0; q < 4; ++q) to[q] = raw8_load((const TX*)p.A + (size_t)min(m0 + i * 16 + q * 4 + g, p.M - 1) * p.K, c, p.K);
+      };
+      fetch(0, next);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const Bf4 ab = to_bf16<FMT>(a[i], b8_scale(ba[i]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) raw[q] = next[q];
+        if (i + 1 < MT) fetch(i + 1, next);
+        int e[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+          raw8_get(raw[q], c, p.K, v);
+          e[q] = b8_exponent_of(b8_max16(b8_mag8(v)), FMT);
+          const int row = i * 16 + q * 4 + g;
+          *reinterpret_cast<u32x2_t*>(mine + row * 128 + (((r16 >> 1) ^ ((row >> 1) & 7)) << 4) + (r16 & 1) * 8) = b8_pack8(v, e[q], FMT);
+        }
+        ba[i] = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int theirs = __shfl(e[q], (r16 & 3) * 16, 64);       // of row i * 16 + 4 q + r16 % 4
+          if ((r16 >> 2) == q) ba[i] = theirs;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) ba[i] = (int)(word_a[i] >> (kb & 3) * 8);
+    }
+    const int bw = (int)(word_w >> (kb & 3) * 8);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    const i32x8_t w = frag(MT);
+    if constexpr (!EXACT) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = mfma8<FMT>(frag(i), w, acc[i], ba[i], bw);
+    } else {
+      const Bf4 wb = to_bf16<SDAMD_E4M3>(w, b8_scale(bw & 255));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const Bf4 ab = to_bf16<FMT>(frag(i), b8_scale(ba[i] & 255));
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ab.q[q], wb.q[q], acc[i], 0, 0, 0);
       }
     }
   }
+  float(*ex)[MT * 16][LD] = reinterpret_cast<float(*)[MT * 16][LD]>(smem);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) ex[wave][i * 16 + g * 4 + e][r16] = acc[i][e];
   __syncthreads();
-  for (int t = threadIdx.x; t < MT * 64; t += 512) {
+  for (int t = threadIdx.x; t < MT * 64; t += 64 * NW) {
     const int row = t >> 2, c = (t & 3) * 4;
     f32x4_t s = *reinterpret_cast<const f32x4_t*>(&ex[0][row][c]);
 #pragma unroll
-    for (int w = 1; w < 8; ++w) s += *reinterpret_cast<const f32x4_t*>(&ex[w][row][c]);
+    for (int w = 1; w < NW; ++w) s += *reinterpret_cast<const f32x4_t*>(&ex[w][row][c]);
     g8_store4<TO>(p, m0 + row, n0 + c, s + g8_bias4(p, n0 + c));
   }
 }
@@ -431,25 +464,31 @@ __global__ __launch_bounds__(512) void gemm8_rows_kernel(G8Args p) {
 // ---------------------------------------------------------------------------------------------
 // host entry points
 // ---------------------------------------------------------------------------------------------
-// Few tiles: the kernel without LDS staging, which also splits K over the waves of a workgroup.  The tile kernel takes
-// 0.65 us a step with few tiles on the chip, 1.3 us in its f32 form (512 x 1280 -> 1280, 40 tiles: 9.3 us, this one 12.0;
-// 20 tiles: 9.1 and 8.6; f32 80 tiles: 16.7 and 22.9, 48 tiles: 8.0 and 6.3).
+// Few tiles: the rows kernel, which splits K over the waves of a workgroup and gives every 16 columns a workgroup; the tile
+// kernel's time is then the length of its walk over K (0.65 us a step, 1.3 us in its f32 form) whatever the tiles.  Its time
+// and the tile kernel's, us: 256 x 1280 -> 1280 (20 tiles) 5.0 and 9.2; 512 x 5120 -> 1280 (40) 15.9 and 32.5; 2048 x 320 -> 320
+// (48) 4.8 and 6.1; 1024 x 1280 -> 1280 (80) 10.4 and 9.6; 2048 x 640 -> 640 (80) 8.1 and 6.5.  f32: 2048 x 640 -> 640 9.0 and
+// 10.2; 1024 x 1280 -> 1280 12.5 and 16.6; 4096 x 320 -> 320 (96) 7.7 and 8.2; 512 x 1280 -> 5120 (160) 22.4 and 17.9.
 static long long g8_tiles(int M, int N, int b) { return (long long)((M + b - 1) / b) * ((N + b - 1) / b); }
 constexpr int G8_MAX_WIDTH = 1 << 24;
-// (planned from one sample's rows under sdamd_set_plan_samples: the two kernels add in different orders; all forms of
-// either give the same bits)
+// (Both planned from one sample's rows under sdamd_set_plan_samples: they decide the order of the sums.  The tile kernel's
+// forms give the same bits.)
+static int g8_row_tiles(int rows) { const int M = plan_rows(rows); return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
 static bool g8_few_rows(int rows, int N, bool exact) {
   const int M = plan_rows(rows);
-  return (M <= 64 || g8_tiles(M, N, 128) < (exact ? 64 : 32)) && (rows + 63) / 64 <= 65535;
+  return (M <= 64 || g8_tiles(M, N, 128) < (exact ? 128 : 64)) && rows / (16 * g8_row_tiles(rows)) < 65535;
 }
-// That kernel can quantise rows on its way.  A wave then quantises its blocks of K for all the workgroup's 16-row tiles, which
-// saves the launch and the buffers of quantising first (9 us of host work a call) and costs more on the GPU the more of
-// them there are: 1 x 320 -> 1280: 3.4 us, first quantised 4.7; 16 x 1280 -> 1280: 5.7 and 6.3; 154 x 768 -> 640 (4 a wave): 9.5
-// and 7.7; 64 x 1280 -> 640 (8): 13.7 and 9.1; 64 x 5120 -> 320 (20): 42 and 18.  So up to 4 a wave.
+// That kernel can quantise rows on its way.  A wave then quantises its blocks of K for all the workgroup's 16-row tiles,
+// every 16 columns anew: no second launch and no buffers for the blocks, half the time of an eager call (64 x 320 -> 1280: 8.7
+// us, first quantised 18.5; 154 x 768 -> 640: 9.8 and 17.6).  On the GPU, us, us first quantised, by the blocks that a compute
+// unit's waves quantise one after the other: 1 x 320 -> 1280 (1) 3.5, 4.8; 16 x 1280 -> 1280 (1) 4.8, 5.6; 32 x 1280 -> 1280 (2)
+// 7.0, 6.1; 64 x 768 -> 640 (4) 8.5, 6.1; 256 x 1024 -> 640 (4) 10.7, 6.7; 64 x 1280 -> 640 (8) 13.4, 7.2; 512 x 320 -> 1280 (12)
+// 22.7, 8.4, and then the eager call loses too (21.9, 17.8).  So up to 4.
 extern "C" int sdamd_linear8_quantises(int M, int N, int K, int out_dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const int tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  return g8_few_rows(M, N, out_dtype == SDAMD_F32) && (b8_kblocks(K) + 7) / 8 * tiles <= 4;
+  const int tiles = g8_row_tiles(M), waves = tiles == 4 ? 8 : 16;
+  const long long groups = (long long)((M + 16 * tiles - 1) / (16 * tiles)) * ((N + 15) / 16);
+  return g8_few_rows(M, N, out_dtype == SDAMD_F32) && (b8_kblocks(K) + waves - 1) / waves * tiles * ((groups + 255) / 256) <= 4;
 }
 
 template <int BM, int BN, int WGM, int WGN, int PLACES, int FMT, bool EXACT, typename TO>
@@ -465,19 +504,27 @@ static int g8_tile_launch(G8Args p, hipStream_t st) {
   return 0;
 }
 
+template <int MT, int FMT, bool EXACT, typename TO, typename TX>
+static int g8_rows_launch(const G8Args& p, dim3 grid, hipStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int lds = g8_rows_lds<MT>();
+  auto k = gemm8_rows_kernel<MT, FMT, EXACT, TO, TX>;
+  const hipError_t e = sd_lds_opt_in(done, (const void*)k, lds);
+  if (e != hipSuccess) return sdamd_set_error(2, "linear8: %s", hipGetErrorString(e));
+  k<<<grid, 64 * g8_rows_waves<MT>(), lds, st>>>(p);
+  return 0;
+}
+
 template <int FMT, bool EXACT, typename TO>
 static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
   if (g8_few_rows(p.M, p.N, EXACT)) {
-    const dim3 grid((p.N + 15) / 16, p.M <= 32 ? 1 : (p.M + 63) / 64);
+    const int mt = g8_row_tiles(p.M);
+    const dim3 grid((p.N + 15) / 16, (p.M + 16 * mt - 1) / (16 * mt));
 #define G8_ROWS(TX)                                                                              \
-  do {                                                                                           \
-    if (p.M <= 16) gemm8_rows_kernel<1, FMT, EXACT, TO, TX><<<grid, 512, 0, st>>>(p);            \
-    else if (p.M <= 32) gemm8_rows_kernel<2, FMT, EXACT, TO, TX><<<grid, 512, 0, st>>>(p);       \
-    else gemm8_rows_kernel<4, FMT, EXACT, TO, TX><<<grid, 512, 0, st>>>(p);                      \
-  } while (0)
-    if (x_dtype == SDAMD_F32) G8_ROWS(float); else if (x_dtype == SDAMD_BF16) G8_ROWS(bf16_t); else G8_ROWS(unsigned char);
+  (mt == 1 ? g8_rows_launch<1, FMT, EXACT, TO, TX>(p, grid, st)                                  \
+           : mt == 2 ? g8_rows_launch<2, FMT, EXACT, TO, TX>(p, grid, st) : g8_rows_launch<4, FMT, EXACT, TO, TX>(p, grid, st))
+    return x_dtype == SDAMD_F32 ? G8_ROWS(float) : x_dtype == SDAMD_BF16 ? G8_ROWS(bf16_t) : G8_ROWS(unsigned char);
 #undef G8_ROWS
-    return 0;
   }
   SD_CHECK(g8_tiles(p.M, p.N, 128) < (1ll << 31), "linear8: too large, M=%d N=%d", p.M, p.N);
   // 256 x 256 where it fills the chip and does not multiply an eighth more padding than 128 x 128 (two workgroups per CU):

@@ -89,8 +89,12 @@ __global__ __launch_bounds__(256) void ln_train_kernel(const TX* __restrict__ x,
         for (int j = 0; j < 8; ++j) if (c + j >= C) v[i + s][j] = 0.f;
         m = max(m, b8_mag8(v[i + s]));
       }
+      if constexpr (G == 8) {
 #pragma unroll
-      for (int o = (G == 8 ? 8 : 16) / 2; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+        for (int o = 4; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+      } else {
+        m = b8_max16(m);
+      }
       const int e = b8_exponent_of(m, out_dtype);
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) {
