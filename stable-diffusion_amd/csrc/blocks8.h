@@ -138,10 +138,12 @@ template <typename T> __device__ __forceinline__ void raw8_get(const Raw8<T>& r,
   }
   if (C % 8 != 0) {                              // (uniform) shift a partial vector down by c - (C - 8)
     const int s = C < 8 ? c : max(c - (C - 8), 0);
+    if (s > 0) {                                 // (one vector of a row: most waves branch over it)
 #pragma unroll
-    for (int b = 4; b > 0; b >>= 1)
+      for (int b = 4; b > 0; b >>= 1)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = s & b ? (j + b < 8 ? v[j + b] : 0.f) : v[j];
+        for (int j = 0; j < 8; ++j) v[j] = s & b ? (j + b < 8 ? v[j + b] : 0.f) : v[j];
+    }
   }
   if (c >= C) {
 #pragma unroll

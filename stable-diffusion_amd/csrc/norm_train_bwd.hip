@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256) void ln_backward_reduce(const float* __restric
 // One launch for both where the column workgroups' walk over all rows is short: they take as long as the rest up to about
 // 1024 rows of 1024 (1024 x 768: 7.3 us, two launches 13.1; 2048 x 768: 18.9 and 14.2; 1024 x 2048: 16.8 and 13.7).
 static bool lnb_one_launch(int rows, int C) { return rows <= 1024 && (long long)rows * C <= (1 << 20); }
-// One workgroup per CU (256; a few more rather than another turn for all): each leaves a row of partial sums and pays for
+// One workgroup per CU (256, never 257: 4099 x 1001 in 171 workgroups of three turns 16.0 us, in 257 of two 19.6): each leaves a row of partial sums and pays for
 // joining its waves' (65536 x 320 bf16: 41.5 us, with 512 workgroups 49.0, with 1024 64.1).
 static int lnb_grid(int rows, int C) {
   const int nvec = (C + 7) / 8;
@@ -291,7 +291,7 @@ static int lnb_grid(int rows, int C) {
 #undef LNB_ROWS
   const int blocks = (rows + rp - 1) / rp;
   if (lnb_one_launch(rows, C)) return blocks;
-  const int turns = (blocks + 267) / 268;
+  const int turns = (blocks + 255) / 256;
   return (blocks + turns - 1) / turns;
 }
 
