@@ -13,10 +13,23 @@
 
 constexpr int LNT_MAX_C = 256 * 6 * 8;
 
+template <int N> __device__ __forceinline__ float rotate16(float v) {
+  return __builtin_bit_cast(float, b8_rotate16<N>(__builtin_bit_cast(unsigned, v)));
+}
 // sum over the G lanes of a row (G = 256, 512: four or eight waves, through LDS; red: a float per wave of the workgroup)
 template <int G> __device__ __forceinline__ float group_sum(float v, float* red) {
+  constexpr int W = G < 64 ? G : 64;
+  if constexpr (W > 32) v += __shfl_xor(v, 32, 64);
+  if constexpr (W > 16) v += __shfl_xor(v, 16, 64);
+  if constexpr (W >= 16) {                       // within 16 lanes by rotations in the vector unit, not through LDS
+    v += rotate16<8>(v);
+    v += rotate16<4>(v);
+    v += rotate16<2>(v);
+    v += rotate16<1>(v);
+  } else {
 #pragma unroll
-  for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  }
   if constexpr (G > 64) {
     const int first = G == 256 ? (threadIdx.x >> 8) * 4 : 0;
     __syncthreads();                             // (red may still be read from the previous call)
