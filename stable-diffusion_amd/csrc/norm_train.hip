@@ -1,8 +1,8 @@
-// LayerNorm forward for training (norm_train.h).  65536 x 320 f32 -> bf16: 21.7 us (5.8 TB/s), -> e4m3 blocks 23.4; 77 x 768: 3.7.
+// LayerNorm forward for training (norm_train.h).  65536 x 320 f32 -> bf16: 21.3 us (5.9 TB/s), -> e4m3 blocks 21.6; 77 x 768: 3.5.
 #include "norm_train.h"
 
 // lanes per row and vectors per lane: at most 4 vectors where the row allows it.  (With 5 or 6 and fewer lanes no lane is
-// idle at 320, 640 and 1280 columns, but each waits longer: 65536 x 320 -> e4m3 31.7 us, 77 x 768 5.2.)
+// idle at 320, 640 and 1280 columns, but each waits longer: 65536 x 320 -> e4m3 31.7 us against 21.6, 77 x 768 5.2 against 3.5.)
 #define LNT_PICK(nvec, CASE)                                                                                          \
   do {                                                                                                                \
     const int nv_ = (nvec);                                                                                           \

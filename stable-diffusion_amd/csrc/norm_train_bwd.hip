@@ -75,7 +75,7 @@ __device__ __forceinline__ void again(RawQ& r) { asm volatile("" : "+v"(r.q)); }
 constexpr int LNB_THREADS = 512;   // two waves per SIMD: one waits for memory while the other computes
 
 // lanes per row and vectors per lane: at most 4, so that the sums of both weight gradients (16 registers a vector), a row and
-// the next fit 256 registers, two waves per SIMD.  (5 vectors a lane, four waves of 400 registers: 65536 x 320 in 41.5 us.)
+// the next fit 256 registers, two waves per SIMD.  (5 vectors a lane, four waves of 400 registers: 65536 x 320 bf16 in 41.5 us, this way 35.5.)
 #define LNB_PICK(nvec, CASE)                                                                                       \
   do {                                                                                                             \
     const int nv_ = (nvec);                                                                                        \
@@ -279,10 +279,10 @@ __global__ __launch_bounds__(256) void ln_backward_reduce(const float* __restric
 }
 
 // One launch for both where the column workgroups' walk over all rows is short: they take as long as the rest up to about
-// 1024 rows of 1024 (1024 x 768: 7.3 us, two launches 13.1; 2048 x 768: 18.9 and 14.2; 1024 x 2048: 16.8 and 13.7).
+// 1024 rows of 1024 (1024 x 768: 6.8 us, two launches 13.1; 2048 x 768: 18.9 and 12.7; 1024 x 2048: 16.8 and 13.7).
 static bool lnb_one_launch(int rows, int C) { return rows <= 1024 && (long long)rows * C <= (1 << 20); }
-// One workgroup per CU (256, never 257: 4099 x 1001 in 171 workgroups of three turns 16.0 us, in 257 of two 19.6): each leaves a row of partial sums and pays for
-// joining its waves' (65536 x 320 bf16: 41.5 us, with 512 workgroups 49.0, with 1024 64.1).
+// One workgroup per CU (256, never 257: 4099 x 1001 in 171 workgroups of three turns 16.0 us, in 257 of two 19.6): each
+// leaves a row of partial sums and pays for joining its waves' (65536 x 320 bf16: 35.5 us, in 384 workgroups 49.2, in 512 42.2).
 static int lnb_grid(int rows, int C) {
   const int nvec = (C + 7) / 8;
   int rp = 1;
