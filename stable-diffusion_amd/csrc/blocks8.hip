@@ -146,8 +146,8 @@ __device__ __forceinline__ void gelu_slope(float x, float& gelu, float& slope) {
   slope = __builtin_fmaf(x * 0.39894228040143267794f, e, cdf);
 }
 
-// ---- GeGLU backward (65536 x 1280 bf16 from e4m3: 130 us = 5.2 TB/s): dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
-// (TH = unsigned char)
+// ---- GeGLU backward: dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
+// (TH = unsigned char).  65536 x 1280 bf16 from e4m3: 130 us = 5.2 TB/s.
 template <typename TD, typename TH, typename TO>
 __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restrict__ dout, const TH* __restrict__ h,
                                                              const unsigned char* __restrict__ scale, TO* __restrict__ dh,
@@ -199,7 +199,7 @@ extern "C" int sdamd_quant8(const void* x, void* q, unsigned char* scale, long l
   SD_CHECK(is_val(dtype) && is_fmt(fmt), "quant8: unsupported dtypes in=%d out=%d", dtype, fmt);
   SD_CHECK(rows > 0 && K > 0 && K <= (1 << 30) && ldx >= 0, "quant8: bad shape rows=%lld K=%d", rows, K);
   const int KB = b8_kblocks(K);
-  SD_CHECK(rows <= (1ll << 40) && rows * (long long)KB < (1ll << 29), "quant8: too large, rows=%lld K=%d", rows, K);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)KB <= (1ll << 29) - 32, "quant8: too large, rows=%lld K=%d", rows, K);
   const unsigned nblk = (unsigned)(rows * KB);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == SDAMD_BF16)
@@ -228,7 +228,7 @@ extern "C" int sdamd_dequant8(const void* q, const unsigned char* scale, void* o
   SD_CHECK(is_val(out_dtype) && is_fmt(fmt), "dequant8: unsupported dtypes in=%d out=%d", fmt, out_dtype);
   SD_CHECK(rows > 0 && K > 0 && K <= (1 << 30) && (block_rows == 1 || block_rows == B8_BLOCK), "dequant8: bad shape rows=%lld K=%d block_rows=%d", rows, K, block_rows);
   const int KB = b8_kblocks(K);
-  SD_CHECK(rows <= (1ll << 40) && rows * (long long)KB < (1ll << 28), "dequant8: too large, rows=%lld K=%d", rows, K);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)KB <= (1ll << 28) - 16, "dequant8: too large, rows=%lld K=%d", rows, K);
   const unsigned nblk = (unsigned)(rows * KB);
   const int shift = block_rows == 1 ? 0 : 7, SP = b8_scale_stride(K);
   hipStream_t st = (hipStream_t)stream;
@@ -257,7 +257,8 @@ static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned ch
 extern "C" int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt, void* stream) {
   SD_CHECK(is_val(dtype) && is_fmt(fmt), "geglu_train: unsupported dtypes h=%d kept=%d", dtype, fmt);
   SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_train: bad shape rows=%lld F=%d", rows, F);
-  SD_CHECK(rows <= (1ll << 40) && rows * (long long)((F + 7) / 8) < (1ll << 31), "geglu_train: too large, rows=%lld F=%d", rows, F);
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)((F + 7) / 8) < (1ll << 31) && (F % B8_BLOCK == 0 || rows * (long long)b8_kblocks(2 * F) <= (1ll << 29) - 32),
+           "geglu_train: too large, rows=%lld F=%d", rows, F);
   if (dtype == SDAMD_BF16) geglu_train_launch<bf16_t>((const bf16_t*)h, (bf16_t*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
   else geglu_train_launch<float>((const float*)h, (float*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
   SD_LAUNCH_CHECK("geglu_train");

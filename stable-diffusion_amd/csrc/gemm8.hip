@@ -481,7 +481,7 @@ constexpr int G8_MAX_WIDTH = 1 << 24;
 static int g8_row_tiles(int rows) { const int M = plan_rows(rows); return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
 static bool g8_few_rows(int rows, int N, bool exact) {
   const int M = plan_rows(rows);
-  return (M <= 64 || g8_tiles(M, N, 128) < (exact ? 128 : 64)) && rows / (16 * g8_row_tiles(rows)) < 65535;
+  return M <= 64 || g8_tiles(M, N, 128) < (exact ? 128 : 64);
 }
 // That kernel can quantise rows on its way.  A wave then quantises its blocks of K for all the workgroup's 16-row tiles,
 // every 16 columns anew: no second launch and no buffers for the blocks, half the time of an eager call (64 x 320 -> 1280: 8.7
@@ -510,13 +510,23 @@ static int g8_tile_launch(G8Args p, hipStream_t st) {
 }
 
 template <int MT, int FMT, bool EXACT, typename TO, typename TX>
-static int g8_rows_launch(const G8Args& p, dim3 grid, hipStream_t st) {
+static int g8_rows_launch(G8Args p, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
   constexpr int lds = g8_rows_lds<MT>();
   auto k = gemm8_rows_kernel<MT, FMT, EXACT, TO, TX>;
   const hipError_t e = sd_lds_opt_in(done, (const void*)k, lds);
   if (e != hipSuccess) return sdamd_set_error(2, "linear8: %s", hipGetErrorString(e));
-  k<<<grid, 64 * g8_rows_waves<MT>(), lds, st>>>(p);
+  constexpr int most = 65535 * 16 * MT;          // rows of a launch (only a planned batch has more)
+  const int rows = p.M;
+  const size_t ldx = sizeof(TX) == 1 ? (size_t)p.KB * B8_BLOCK : (size_t)p.K * sizeof(TX), ldo = (size_t)p.N * sizeof(TO);
+  for (int m = 0; m < rows; m += p.M) {
+    p.M = min(most, rows - m);
+    k<<<dim3((p.N + 15) / 16, (p.M + 16 * MT - 1) / (16 * MT)), 64 * g8_rows_waves<MT>(), lds, st>>>(p);
+    p.A = (const char*)p.A + (size_t)p.M * ldx;
+    if (p.As) p.As += (size_t)p.M * p.SP;
+    p.out = (char*)p.out + (size_t)p.M * ldo;
+    if (p.residual) p.residual = (const char*)p.residual + (size_t)p.M * ldo;
+  }
   return 0;
 }
 
@@ -524,10 +534,9 @@ template <int FMT, bool EXACT, typename TO>
 static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
   if (g8_few_rows(p.M, p.N, EXACT)) {
     const int mt = g8_row_tiles(p.M);
-    const dim3 grid((p.N + 15) / 16, (p.M + 16 * mt - 1) / (16 * mt));
 #define G8_ROWS(TX)                                                                              \
-  (mt == 1 ? g8_rows_launch<1, FMT, EXACT, TO, TX>(p, grid, st)                                  \
-           : mt == 2 ? g8_rows_launch<2, FMT, EXACT, TO, TX>(p, grid, st) : g8_rows_launch<4, FMT, EXACT, TO, TX>(p, grid, st))
+  (mt == 1 ? g8_rows_launch<1, FMT, EXACT, TO, TX>(p, st)                                  \
+           : mt == 2 ? g8_rows_launch<2, FMT, EXACT, TO, TX>(p, st) : g8_rows_launch<4, FMT, EXACT, TO, TX>(p, st))
     return x_dtype == SDAMD_F32 ? G8_ROWS(float) : x_dtype == SDAMD_BF16 ? G8_ROWS(bf16_t) : G8_ROWS(unsigned char);
 #undef G8_ROWS
   }

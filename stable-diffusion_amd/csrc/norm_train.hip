@@ -127,7 +127,7 @@ extern "C" int sdamd_layernorm_train(const void* x, void* y, unsigned char* y_sc
            "layernorm_train: unsupported dtypes in=%d out=%d", dtype, out_dtype);
   SD_CHECK(out_dtype < SDAMD_E4M3 || y_scale, "layernorm_train: 8-bit output without room for its scales");
   SD_CHECK(rows > 0 && C > 0 && C <= LNT_MAX_C, "layernorm_train: unsupported shape rows=%d C=%d (C <= %d)", rows, C, LNT_MAX_C);
-  SD_CHECK(rows < (1 << 24) || (rows < (1 << 27) && C <= 512), "layernorm_train: too many rows, %d of %d", rows, C);   // (a launch's 2^32 threads)
+  SD_CHECK(rows < (1 << 24) || (rows <= (1 << 27) - 32 && C <= 512), "layernorm_train: too many rows, %d of %d", rows, C);   // (a launch's 2^32 threads)
   if (dtype == SDAMD_BF16) ln_train_launch<bf16_t>(x, y, y_scale, gamma, beta, mean, rstd, rows, C, eps, out_dtype, (hipStream_t)stream);
   else ln_train_launch<float>(x, y, y_scale, gamma, beta, mean, rstd, rows, C, eps, out_dtype, (hipStream_t)stream);
   SD_LAUNCH_CHECK("layernorm_train");

@@ -227,6 +227,37 @@ def test_linear8_large_tile(out):
     close(got, want, linear_tol(xq, wq, np.abs(xq) @ np.abs(wq).T, out, want, 0), "large")
 
 
+@pytest.mark.parametrize("M,K,N", [(256, 640, 640), (1000, 200, 640), (1500, 257, 2050), (2048, 130, 2304), (4100, 260, 3501), (4096, 128, 4096)])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_linear8_epilogues_of_every_kernel(M, K, N, out):
+    """Bias, residual and activation together at sizes that reach each kernel, with whole tiles and ragged ones; the residual
+    may be the output."""
+    x, w = rnd(3, (M, K), BF16), rnd(4, (N, K), scale=K ** -0.5)
+    bias, res = rnd(5, (N,)), rnd(6, (M, N), out)
+    xq, wq = blocks_ref(np64(x), E4M3)[0], blocks_ref(np64(w), E4M3, 128)[0]
+    wb, bd = ops.quantize8_weight(w.to(DEV)), bias.to(DEV)
+    for b, r, act in ((bias, res, ops.ACT_SILU), (None, res, ops.ACT_NONE), (bias, None, ops.ACT_NONE), (None, None, ops.ACT_QUICK_GELU)):
+        want, mag = linear_ref(xq, wq, b, r, act)
+        io = None if r is None else r.to(DEV)
+        got = ops.linear8(x.to(DEV), wb, None if b is None else bd, io, act, out, out=io)
+        close(got, want, linear_tol(xq, wq, mag, out, want, act), f"bias {b is not None} residual {r is not None} act {act}")
+
+
+def test_linear8_planned_batch_of_many_samples():
+    """Few rows a sample, more in all than one launch of the rows kernel takes."""
+    S, R, K, N = 131100, 8, 8, 16
+    x, w = rnd(3, (S * R, K)).to(DEV), ops.quantize8_weight(rnd(4, (N, K)).to(DEV))
+    res = rnd(5, (S * R, N)).to(DEV)
+    with ops.plan_samples(S):
+        for xx in (x, ops.quantize8(x)):
+            batch = ops.linear8(xx, w, residual=res)
+            for s in (0, 131070, 131099):
+                rows = slice(s * R, s * R + R)
+                with ops.plan_samples(1):
+                    alone = ops.linear8(x[rows], w, residual=res[rows])
+                assert torch.equal(batch[rows], alone)
+
+
 def test_linear8_scale_range():
     """Blocks of very different size in one row, tiny ones and huge ones: the scales do the work."""
     M, K, N = 40, 640, 96
@@ -268,10 +299,12 @@ def test_linear8_shapes_out_and_refusals():
     assert torch.equal(ops.linear8(strided[:, 7:207], w), ops.linear8(strided[:, 7:207].contiguous(), w))
     assert torch.equal(ops.linear8(strided[:4, 7:207], w), ops.linear8(strided[:4, 7:207].contiguous(), w))
     assert ops.linear8(torch.empty(0, 200, device=DEV), w).shape == (0, 48)
+    square = torch.zeros(64, 64, device=DEV)
     bad = [lambda: ops.linear8(x, x), lambda: ops.linear8(x[..., :100], w), lambda: ops.linear8(x, w, bias=torch.zeros(47, device=DEV)),
            lambda: ops.linear8(x, w, bias=torch.zeros(48, device=DEV, dtype=BF16)),
            lambda: ops.linear8(x, w, residual=torch.zeros(2, 5, 48, device=DEV), out_dtype=BF16),
            lambda: ops.linear8(x, w, act=ops.ACT_GEGLU), lambda: ops.linear8(x, w, out=buf[:1]), lambda: ops.linear8(w, w),
+           lambda: ops.linear8(square, ops.quantize8_weight(square), out=square),
            lambda: ops.linear8(x.cpu(), w)]
     for call in bad:
         with pytest.raises(_lib.SdamdError):

@@ -59,6 +59,14 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
 
 
+def test_c_boundary_keeps_launches_below_2_to_32_threads():
+    refused(L.sdamd_quant8(P, P, P, (1 << 29) - 31, 8, 8, 0, 2, 0), "too large")
+    refused(L.sdamd_dequant8(P, P, P, (1 << 28) - 15, 8, 1, 2, 0, 0), "too large")
+    refused(L.sdamd_geglu_train(P, P, P, P, 1 << 30, 4, 0, 2, 0), "too large")
+    refused(L.sdamd_geglu_train(P, P, P, P, 1 << 30, 128, 0, 2, 0), "too large")
+    refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, (1 << 27) - 31, 512, 1e-5, 0, 0, 0), "too many rows")
+
+
 def test_python_refuses_the_cpu_and_bad_blocks():
     x = torch.zeros(4, 200)
     for call in (lambda: ops.quantize8(x), lambda: ops.quantize8_weight(x), lambda: ops.layernorm_train(x, x[0], x[0]),
