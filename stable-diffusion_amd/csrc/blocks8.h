@@ -154,22 +154,31 @@ template <typename T> __device__ __forceinline__ void row_load8(const T* row, in
   const Raw8<T> r = raw8_load(row, c, C);
   raw8_get(r, c, C, v);
 }
-// store the n (<= 8, may be <= 0) values that belong to the row
-__device__ __forceinline__ void row_store8(float* p, int n, const float (&v)[8]) {
+// Results of half the last-level cache (256 MB) or more are written past it: whoever reads them next finds the larger part
+// gone anyway, and the lines they would push out are the operands'.  (Alone, operands and results from rotating buffers: 36864 x
+// 1280 -> 10240, 755 MB: 497 us kept, 473 past; 16384 x 640 -> 5120, 168 MB: 73.9 and 62.6, with the GeGLU that reads it
+// 132.7 and 135.8; 65536 x 320 -> 2560, 336 MB, with its GeGLU 241 and 234; 4096 x 1280 -> 10240, 84 MB, with its GeGLU 93.1
+// and 104.3: so not the smaller ones.)
+static inline bool b8_past_cache(double bytes) { return bytes >= 134217728.0; }
+// store the n (<= 8, may be <= 0) values that belong to the row; PAST: past the cache (a template argument: the compiler joins the two stores of a branch into a plain one)
+template <bool PAST = false> __device__ __forceinline__ void row_store8(float* p, int n, const float (&v)[8]) {
   if (n >= 8) {
-    *reinterpret_cast<b8_f32x4_a4*>(p) = (f32x4_t){v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<b8_f32x4_a4*>(p + 4) = (f32x4_t){v[4], v[5], v[6], v[7]};
+    const f32x4_t lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+    b8_f32x4_a4* d = reinterpret_cast<b8_f32x4_a4*>(p);
+    if constexpr (PAST) { __builtin_nontemporal_store(lo, d); __builtin_nontemporal_store(hi, reinterpret_cast<b8_f32x4_a4*>(p + 4)); }
+    else { *d = lo; *reinterpret_cast<b8_f32x4_a4*>(p + 4) = hi; }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) if (j < n) p[j] = v[j];
   }
 }
-__device__ __forceinline__ void row_store8(bf16_t* p, int n, const float (&v)[8]) {
+template <bool PAST = false> __device__ __forceinline__ void row_store8(bf16_t* p, int n, const float (&v)[8]) {
   if (n >= 8) {
     u32x4_t t;
 #pragma unroll
     for (int i = 0; i < 4; ++i) t[i] = pack_bf2(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<b8_u32x4_a2*>(p) = t;
+    if constexpr (PAST) __builtin_nontemporal_store(t, reinterpret_cast<b8_u32x4_a2*>(p));
+    else *reinterpret_cast<b8_u32x4_a2*>(p) = t;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) if (j < n) p[j] = f2bf(v[j]);

@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void dequant8_kernel(const unsigned char* __re
 // ---- GeGLU that keeps its input in 8 bits: h [rows][2F] -> out [rows][F] = value * gelu(gate), and h's blocks.
 // 65536 x 1280 bf16: 119 us = 5.6 TB/s.
 // F % 128 == 0: the 16 lanes that hold a value block hold the gate block of the same columns too, so h is read once.
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned char* __restrict__ q,
                                                           unsigned char* __restrict__ scale, unsigned nblk, int FB, int SP, int fmt) {
   const int sub = threadIdx.x & 15;
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ 
   if (b >= nblk) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
-  row_store8(out + (size_t)bb * B8_BLOCK + sub * 8, 8, o);
+  row_store8<PAST>(out + (size_t)bb * B8_BLOCK + sub * 8, 8, o);
   *reinterpret_cast<u32x2_t*>(q + vb * B8_BLOCK + sub * 8) = b8_pack8(v, ev, fmt);
   *reinterpret_cast<u32x2_t*>(q + gb * B8_BLOCK + sub * 8) = b8_pack8(g, eg, fmt);
   if (sub == 0) { scale[(size_t)row * SP + fb] = (unsigned char)ev; scale[(size_t)row * SP + FB + fb] = (unsigned char)eg; }
@@ -148,7 +148,7 @@ __device__ __forceinline__ void gelu_slope(float x, float& gelu, float& slope) {
 
 // ---- GeGLU backward: dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
 // (TH = unsigned char).  65536 x 1280 bf16 from e4m3: 130 us = 5.2 TB/s.
-template <typename TD, typename TH, typename TO>
+template <typename TD, typename TH, typename TO, bool PAST>
 __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restrict__ dout, const TH* __restrict__ h,
                                                              const unsigned char* __restrict__ scale, TO* __restrict__ dh,
                                                              unsigned nvec, int VR, int F, int ldh, int SP, int fmt) {
@@ -185,8 +185,8 @@ __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restric
     dv[j] = d[j] * ge;
     dg[j] = d[j] * v[j] * sl;
   }
-  row_store8(dh + (size_t)row * 2 * F + c, F - c, dv);
-  row_store8(dh + (size_t)row * 2 * F + F + c, F - c, dg);
+  row_store8<PAST>(dh + (size_t)row * 2 * F + c, F - c, dv);
+  row_store8<PAST>(dh + (size_t)row * 2 * F + F + c, F - c, dg);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -245,7 +245,8 @@ static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned ch
   const int SP = b8_scale_stride(2 * F);
   if (F % B8_BLOCK == 0) {
     const unsigned nblk = (unsigned)(rows * (F / B8_BLOCK));
-    geglu_train_kernel<T><<<(nblk + 15) / 16, 256, 0, st>>>(h, out, q, scale, nblk, F / B8_BLOCK, SP, fmt);
+    auto k = b8_past_cache((double)rows * F * sizeof(T)) ? geglu_train_kernel<T, true> : geglu_train_kernel<T, false>;
+    k<<<(nblk + 15) / 16, 256, 0, st>>>(h, out, q, scale, nblk, F / B8_BLOCK, SP, fmt);
   } else {
     const int KB = b8_kblocks(2 * F), VR = (F + 7) / 8;
     const unsigned nblk = (unsigned)(rows * KB), nvec = (unsigned)(rows * VR);
@@ -276,8 +277,10 @@ extern "C" int sdamd_geglu_backward(const void* dout, const void* h, const unsig
   const unsigned nvec = (unsigned)(rows * VR);
   hipStream_t st = (hipStream_t)stream;
   const int SP = b8_scale_stride(2 * F), ldq = b8_kblocks(2 * F) * B8_BLOCK;
+  const bool past = b8_past_cache((double)rows * 2 * F * (dh_dtype == SDAMD_F32 ? 4 : 2));
 #define GB_LAUNCH(TD, TH, TO, LD) \
-  geglu_backward_kernel<TD, TH, TO><<<(nvec + 255) / 256, 256, 0, st>>>((const TD*)dout, (const TH*)h, h_scale, (TO*)dh, nvec, VR, F, LD, SP, h_dtype)
+  (past ? geglu_backward_kernel<TD, TH, TO, true> : geglu_backward_kernel<TD, TH, TO, false>)<<<(nvec + 255) / 256, 256, 0, st>>>( \
+      (const TD*)dout, (const TH*)h, h_scale, (TO*)dh, nvec, VR, F, LD, SP, h_dtype)
 #define GB_H(TD, TO) \
   { if (h_dtype == SDAMD_F32) GB_LAUNCH(TD, float, TO, 2 * F); else if (h_dtype == SDAMD_BF16) GB_LAUNCH(TD, bf16_t, TO, 2 * F); else GB_LAUNCH(TD, unsigned char, TO, ldq); }
   if (dout_dtype == SDAMD_F32) { if (dh_dtype == SDAMD_F32) GB_H(float, float) else GB_H(float, bf16_t) }

@@ -29,6 +29,7 @@ struct G8Args {
   const void* residual;
   int M, N, K, KB, SP, act;
   int tiles_m, tiles_n;
+  bool past;                       // the result goes past the cache
 };
 
 // one 128-wide step of a 16 x 16 tile
@@ -259,6 +260,10 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
       if constexpr (sizeof(TO) == 4) *reinterpret_cast<g8_f32x4_a4*>(out + lo) = v;
       else *reinterpret_cast<g8_u32x2_a2*>(out + lo) = (u32x2_t){pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
     };
+    auto put_past = [&](f32x4_t v) {
+      if constexpr (sizeof(TO) == 4) __builtin_nontemporal_store(v, reinterpret_cast<g8_f32x4_a4*>(out + lo));
+      else __builtin_nontemporal_store((u32x2_t){pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])}, reinterpret_cast<g8_u32x2_a2*>(out + lo));
+    };
     // the next row; the assembly keeps the compiler from working out all rows' addresses ahead of time (registers)
     auto down = [&](int e) {
       out += e == 3 ? 13 * ld : ld;
@@ -269,6 +274,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
       }
     };
     if (!res && !p.act && tm0 + BM <= p.M && tn0 + BN <= p.N) {
+      branch();
+      if (p.past) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { put_past(value(i, e)); down(e); }
+        return;
+      }
       branch();
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -561,7 +574,8 @@ extern "C" int sdamd_linear8(const void* x, const unsigned char* x_scale, const 
   SD_CHECK(x_dtype < SDAMD_E4M3 || x_scale, "linear8: 8-bit rows without their scales");
   SD_CHECK((((uintptr_t)w | (x_dtype >= SDAMD_E4M3 ? (uintptr_t)x : 0)) & 15) == 0 && (((uintptr_t)w_scale | (uintptr_t)x_scale) & 3) == 0,
            "linear8: blocks have to be 16-byte aligned, their scales 4-byte aligned");
-  G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0};
+  G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0,
+           b8_past_cache((double)M * N * (out_dtype == SDAMD_F32 ? 4 : 2))};
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (out_dtype == SDAMD_F32) rc = fmt == SDAMD_E4M3 ? g8_launch<SDAMD_E4M3, true, float>(p, x_dtype, st) : g8_launch<SDAMD_E5M2, true, float>(p, x_dtype, st);

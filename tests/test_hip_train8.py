@@ -680,6 +680,26 @@ def test_feed_forward_step_on_another_stream_and_in_graphs():
             assert all(torch.equal(x, y) for x, y in zip(res, want)) and all(torch.equal(x, y) for x, y in zip(eager, want_a))
 
 
+def test_results_past_the_cache_are_the_same():
+    """Results of 128 MB or more are written another way than small ones: the same bits as in parts."""
+    w = ops.quantize8_weight(rnd(4, (4100, 130)).to(DEV))
+    for out, M in ((BF16, 16500), (F32, 8250)):
+        x = ops.quantize8(rnd(3, (M, 130)).to(DEV))
+        whole = ops.linear8(x, w, out_dtype=out)
+        assert whole.numel() * whole.element_size() >= 1 << 27
+        for at in range(0, M, M // 3):
+            part = ops.Blocks8(x.q[at:at + M // 3], x.scale[at:at + M // 3], (M // 3, 130))
+            assert torch.equal(whole[at:at + M // 3], ops.linear8(part, w, out_dtype=out))
+    for F, rows in ((1280, 52500), (129, 260400)):
+        h, d = rnd(1, (rows, 2 * F)).to(DEV), rnd(2, (rows, F)).to(DEV)
+        out, kept = ops.geglu_train(h)
+        dh = ops.geglu_backward(d, kept)
+        for at in (0, rows - 500):
+            o, k = ops.geglu_train(h[at:at + 500])
+            assert torch.equal(out[at:at + 500], o) and torch.equal(kept.q[at:at + 500].view(torch.uint8), k.q.view(torch.uint8))
+            assert torch.equal(dh[at:at + 500], ops.geglu_backward(d[at:at + 500], k))
+
+
 def test_writes_stay_inside():
     """Outputs cut from one buffer with guard values on both sides: nothing outside them is written."""
     def guarded(n, dtype):
