@@ -14,6 +14,7 @@
 // the whole block.
 #include "blocks8.h"
 #include "gemm_common.h"
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) void lds_void8_t;
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
@@ -29,7 +30,6 @@ struct G8Args {
   const void* residual;
   int M, N, K, KB, SP, act;
   int tiles_m, tiles_n;
-  bool past;                       // the result goes past the cache
 };
 
 // one 128-wide step of a 16 x 16 tile
@@ -139,7 +139,8 @@ __device__ __forceinline__ void dma4(const void* base, unsigned off, void* lds) 
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(l), "v"(off), "s"(base) : "memory", "m0");
 }
 
-template <int BM, int BN, int WGM, int WGN, int FMT, bool EXACT, typename TO>
+// PAST: the result goes past the cache (b8_past_cache)
+template <int BM, int BN, int WGM, int WGN, int FMT, bool EXACT, typename TO, bool PAST>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
   constexpr int NW = WGM * WGN, TM = BM / WGM / 16, TN = BN / WGN / 16;
   constexpr int STAGE = (BM + BN) * 128, NI = (BM + BN) / 8 / NW;          // DMA instructions of 8 rows per wave and step
@@ -254,34 +255,33 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
     auto branch = [&]() { asm volatile("" : "+v"(bias)); };
     const size_t ld = (size_t)p.N * sizeof(TO), at = (size_t)(tm0 + wm * TM * 16) * ld + (size_t)tn0 * sizeof(TO);
     char* out = (char*)p.out + at;
-    const char* res = p.residual ? (const char*)p.residual + at : nullptr;
     const unsigned lo = (unsigned)(g * 4) * (unsigned)ld + (unsigned)(wn * 64 + r16 * 4) * (unsigned)sizeof(TO);
     auto put = [&](f32x4_t v) {
-      if constexpr (sizeof(TO) == 4) *reinterpret_cast<g8_f32x4_a4*>(out + lo) = v;
-      else *reinterpret_cast<g8_u32x2_a2*>(out + lo) = (u32x2_t){pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
-    };
-    auto put_past = [&](f32x4_t v) {
-      if constexpr (sizeof(TO) == 4) __builtin_nontemporal_store(v, reinterpret_cast<g8_f32x4_a4*>(out + lo));
-      else __builtin_nontemporal_store((u32x2_t){pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])}, reinterpret_cast<g8_u32x2_a2*>(out + lo));
+      auto write = [](auto x, auto* to) {
+        if constexpr (PAST) __builtin_nontemporal_store(x, to);
+        else *to = x;
+      };
+      if constexpr (sizeof(TO) == 4) write(v, reinterpret_cast<g8_f32x4_a4*>(out + lo));
+      else write((u32x2_t){pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])}, reinterpret_cast<g8_u32x2_a2*>(out + lo));
     };
     // the next row; the assembly keeps the compiler from working out all rows' addresses ahead of time (registers)
+    auto next = [&](const char*& at, int e) {
+      at += e == 3 ? 13 * ld : ld;
+      asm volatile("" : "+s"(at));
+    };
     auto down = [&](int e) {
       out += e == 3 ? 13 * ld : ld;
       asm volatile("" : "+s"(out));
-      if (res) {
-        res += e == 3 ? 13 * ld : ld;
-        asm volatile("" : "+s"(res));
+    };
+    auto activate = [&](f32x4_t& v) {
+      if (p.act) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = g8_act(v[j], p.act);
       }
     };
-    if (!res && !p.act && tm0 + BM <= p.M && tn0 + BN <= p.N) {
-      branch();
-      if (p.past) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { put_past(value(i, e)); down(e); }
-        return;
-      }
+    const bool whole = tm0 + BM <= p.M && tn0 + BN <= p.N;
+    const int cols = p.N - n;                              // of the lane's four (<= 0: none)
+    if (!p.residual && !p.act && whole) {
       branch();
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -289,38 +289,84 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm8_kernel(G8Args p) {
         for (int e = 0; e < 4; ++e) { put(value(i, e)); down(e); }
       return;
     }
-    branch();
-    const int cols = p.N - n;                              // of the lane's four (<= 0: none)
+    // The residual is requested as a whole before the first store; it takes the registers of the fragments.  (Each row's
+    // before its store, 16384 x 640 -> 5120: 175 us instead of 106.)  A lane without four columns, or a row, of its own reads elsewhere.
+    typedef typename std::conditional<sizeof(TO) == 4, f32x4_t, u32x2_t>::type raw_t;
+    typedef typename std::conditional<sizeof(TO) == 4, g8_f32x4_a4, g8_u32x2_a2>::type raw_at_t;
+    raw_t rr[TM][4];
+    auto fetch = [&](auto masked) {
+      const char* res = (const char*)p.residual + at;
+      int rows = left;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      asm volatile("" : "+v"(left));                       // (32 masks at once would take 64 scalar registers)
+      for (int i = 0; i < TM; ++i) {
+        asm volatile("" : "+v"(rows));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f32x4_t v = value(i, e);
-        if (e < left && cols > 0) {
-          const TO* r = (const TO*)(res + lo);
-          TO* o = (TO*)(out + lo);
-          if (res) {
-            if (cols >= 4) v += g8_load4(r);
-            else {
+        for (int e = 0; e < 4; ++e) {
+          const char* from = res + lo;
+          if constexpr (decltype(masked)::value) from = e < rows && cols >= 4 ? from : (const char*)p.residual;
+          rr[i][e] = *reinterpret_cast<const raw_at_t*>(from);
+          next(res, e);
+        }
+        rows -= 16;
+      }
+    };
+    auto add = [&](f32x4_t& v, const raw_t& r) {
+      if constexpr (sizeof(TO) == 4) v += r;
+      else v += (f32x4_t){__builtin_bit_cast(float, r[0] << 16), __builtin_bit_cast(float, r[0] & 0xffff0000u),
+                          __builtin_bit_cast(float, r[1] << 16), __builtin_bit_cast(float, r[1] & 0xffff0000u)};
+    };
+    if (whole) {
+      auto run = [&](auto with_residual) {
+        constexpr bool R = decltype(with_residual)::value;
+        if constexpr (R) fetch(std::false_type{});
+        branch();
 #pragma unroll
-              for (int j = 0; j < 3; ++j) if (j < cols) v[j] += Cvt<TO>::ld(r + j);
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f32x4_t v = value(i, e);
+            if constexpr (R) add(v, rr[i][e]);
+            activate(v);
+            put(v);
+            down(e);
+          }
+      };
+      if (p.residual) run(std::true_type{}); else run(std::false_type{});
+      return;
+    }
+    auto run = [&](auto with_residual) {
+      constexpr bool R = decltype(with_residual)::value;
+      if constexpr (R) fetch(std::true_type{});
+      branch();
+      const char* res = (const char*)p.residual + at;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        asm volatile("" : "+v"(left));                     // (32 masks at once would take 64 scalar registers)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f32x4_t v = value(i, e);
+          if (e < left && cols > 0) {
+            if (cols >= 4) {
+              if constexpr (R) add(v, rr[i][e]);
+              activate(v);
+              put(v);
+            } else {
+              if constexpr (R) {
+#pragma unroll
+                for (int j = 0; j < 3; ++j) if (j < cols) v[j] += Cvt<TO>::ld((const TO*)(res + lo) + j);
+              }
+              activate(v);
+#pragma unroll
+              for (int j = 0; j < 3; ++j) if (j < cols) Cvt<TO>::st((TO*)(out + lo) + j, v[j]);
             }
           }
-          if (p.act) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = g8_act(v[j], p.act);
-          }
-          if (cols >= 4) put(v);
-          else {
-#pragma unroll
-            for (int j = 0; j < 3; ++j) if (j < cols) Cvt<TO>::st(o + j, v[j]);
-          }
+          down(e);
+          if constexpr (R) next(res, e);
         }
-        down(e);
+        left -= 16;
       }
-      left -= 16;
-    }
+    };
+    if (p.residual) run(std::true_type{}); else run(std::false_type{});
   };
 
   int t = blockIdx.x / 8;
@@ -511,10 +557,11 @@ extern "C" int sdamd_linear8_quantises(int M, int N, int K, int out_dtype) {
 
 template <int BM, int BN, int WGM, int WGN, int PLACES, int FMT, bool EXACT, typename TO>
 static int g8_tile_launch(G8Args p, hipStream_t st) {
-  static std::atomic<unsigned long long> done{0};
+  static std::atomic<unsigned long long> done[2]{};
   constexpr int lds = 2 * ((BM + BN) * 128 + BM * 4) + 2 * BN * 4;
-  auto k = gemm8_kernel<BM, BN, WGM, WGN, FMT, EXACT, TO>;
-  const hipError_t e = sd_lds_opt_in(done, (const void*)k, lds);
+  const bool past = b8_past_cache((double)p.M * p.N * sizeof(TO));
+  auto k = past ? gemm8_kernel<BM, BN, WGM, WGN, FMT, EXACT, TO, true> : gemm8_kernel<BM, BN, WGM, WGN, FMT, EXACT, TO, false>;
+  const hipError_t e = sd_lds_opt_in(done[past], (const void*)k, lds);
   if (e != hipSuccess) return sdamd_set_error(2, "linear8: %s", hipGetErrorString(e));
   p.tiles_m = (p.M + BM - 1) / BM;
   p.tiles_n = (p.N + BN - 1) / BN;
@@ -574,8 +621,7 @@ extern "C" int sdamd_linear8(const void* x, const unsigned char* x_scale, const 
   SD_CHECK(x_dtype < SDAMD_E4M3 || x_scale, "linear8: 8-bit rows without their scales");
   SD_CHECK((((uintptr_t)w | (x_dtype >= SDAMD_E4M3 ? (uintptr_t)x : 0)) & 15) == 0 && (((uintptr_t)w_scale | (uintptr_t)x_scale) & 3) == 0,
            "linear8: blocks have to be 16-byte aligned, their scales 4-byte aligned");
-  G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0,
-           b8_past_cache((double)M * N * (out_dtype == SDAMD_F32 ? 4 : 2))};
+  G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0};
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (out_dtype == SDAMD_F32) rc = fmt == SDAMD_E4M3 ? g8_launch<SDAMD_E4M3, true, float>(p, x_dtype, st) : g8_launch<SDAMD_E5M2, true, float>(p, x_dtype, st);
