@@ -738,13 +738,18 @@ def _code8(dtype):
     return _FMT8[dtype]
 
 
-# the current device's number and a stream's handle without the Python objects around them (2 us a call)
+# the current device's number and a stream's handle without the Python objects around them (2 us a call); results come from
+# new_empty (1.2 us against 1.6 of torch.empty with a device)
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+_entry = {}              # C entry points by name
 
 
 def _call(device, name, args):
     """One C-ABI call on the tensors' device and its current stream, whatever the current device is."""
-    fn, i = getattr(_lib.lib(), name), device.index
+    fn = _entry.get(name) or _entry.setdefault(name, getattr(_lib.lib(), name))
+    i = device.index
     if i == _current_device():
         rc = fn(*args, _raw_stream(i))
     else:
@@ -833,18 +838,20 @@ class Blocks8:
         out = torch.empty(self.shape, dtype=dtype, device=dev)
         code, K = _code(dtype), self.shape[-1]
         if out.numel():
-            _run8(dev, "sdamd_dequant8", (_p(self.q), _p(self.scale), _p(out), self.q.shape[0], K, self.block_rows, _code8(self.dtype), code),
+            _run8(dev, "sdamd_dequant8", (self.q.data_ptr(), self.scale.data_ptr(), out.data_ptr(), self.q.shape[0], K, self.block_rows, _code8(self.dtype), code),
                   lambda: ("dequantize8", out.numel() * (1 + out.element_size()), f"rows{self.q.shape[0]} K{K}", 0.0))
         return out
 
 
-def _blocks8_empty(shape, dtype, device):
-    """Uninitialised activation blocks for the kernels to fill."""
-    rows, kb = math.prod(shape[:-1]), -(-shape[-1] // BLOCK8)
+def _blocks8_empty(x, dtype):
+    """Uninitialised blocks of x's shape for the kernels to fill."""
+    shape = tuple(x.shape)
+    K = shape[-1]
+    rows, kb = x.numel() // K, -(-K // BLOCK8)
     b = Blocks8.__new__(Blocks8)
-    b.q = torch.empty((rows, kb * BLOCK8), dtype=dtype, device=device)
-    b.scale = torch.empty((rows, -(-kb // 4) * 4), dtype=torch.uint8, device=device)
-    b.shape, b.block_rows = tuple(shape), 1
+    b.q = x.new_empty((rows, kb * BLOCK8), dtype=dtype)
+    b.scale = x.new_empty((rows, -(-kb // 4) * 4), dtype=torch.uint8)
+    b.shape, b.block_rows = shape, 1
     return b
 
 
@@ -858,11 +865,11 @@ def quantize8(x, dtype=torch.float8_e4m3fn):
         raise _lib.SdamdError("quantize8: shape %s, strides %s" % (tuple(x.shape), tuple(x.stride())))
     K = x.shape[-1]
     _fits("quantize8", K)
-    out = _blocks8_empty(x.shape, dtype, dev)
+    out = _blocks8_empty(x, dtype)
     rows = out.q.shape[0]
     if rows:
         ldx = K if x.is_contiguous() else x.stride(0)
-        _run8(dev, "sdamd_quant8", (_p(x), _p(out.q), _p(out.scale), rows, K, ldx, code, fmt),
+        _run8(dev, "sdamd_quant8", (x.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(), rows, K, ldx, code, fmt),
               lambda: ("quantize8", x.numel() * (x.element_size() + 1), f"rows{rows} K{K}", 0.0))
     return out
 
@@ -879,7 +886,7 @@ def quantize8_weight(w):
     kb = -(-K // BLOCK8)
     q = torch.empty((N, kb * BLOCK8), dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty((-(-N // BLOCK8), -(-kb // 4) * 4), dtype=torch.uint8, device=dev)
-    _run8(dev, "sdamd_quant8_weight", (_p(w), _p(q), _p(scale), N, K, w.stride(0), w.stride(1), code),
+    _run8(dev, "sdamd_quant8_weight", (w.data_ptr(), q.data_ptr(), scale.data_ptr(), N, K, w.stride(0), w.stride(1), code),
           lambda: ("quantize8_weight", w.numel() * (w.element_size() + 1), f"N{N} K{K}", 0.0))
     return Blocks8(q, scale, (N, K), BLOCK8)
 
@@ -906,7 +913,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     if act not in (ACT_NONE, ACT_QUICK_GELU, ACT_SILU):
         raise _lib.SdamdError("linear8: unsupported activation %s" % (act,))
     shape = tuple(x.shape[:-1]) + (N,)
-    M = math.prod(shape[:-1])
+    M = xt.shape[0] if is8 else xt.numel() // K
     _fits("linear8", M, N, K)
     if bias is not None:
         _vec_f32("linear8", "bias", bias, N)
@@ -914,7 +921,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
         if not (residual.dtype == out_dtype and residual.is_contiguous() and tuple(residual.shape) == shape):
             raise _lib.SdamdError("linear8: residual %s %s has to be a contiguous %s %s" % (residual.dtype, tuple(residual.shape), out_dtype, shape))
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        out = xt.new_empty(shape, dtype=out_dtype)
     elif not (out.dtype == out_dtype and out.is_contiguous() and tuple(out.shape) == shape):
         raise _lib.SdamdError("linear8: out %s %s has to be a contiguous %s %s" % (out.dtype, tuple(out.shape), out_dtype, shape))
     elif M and out.data_ptr() == xt.data_ptr():
@@ -932,7 +939,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
             is8, xcode = True, f8
     if is8:
         xp, sp = x.q, x.scale
-    _run8(dev, "sdamd_linear8", (_p(xp), _p(sp), _p(w.q), _p(w.scale), _p(out), _p(bias), _p(residual), M, N, K, int(act), xcode, f8, code),
+    _run8(dev, "sdamd_linear8", (xp.data_ptr(), _p(sp), w.q.data_ptr(), w.scale.data_ptr(), out.data_ptr(), _p(bias), _p(residual), M, N, K, int(act), xcode, f8, code),
           lambda: (f"linear8_{_dt(out_dtype)}", 2.0 * M * N * K, f"M{M} N{N} K{K}",
                    M * K * xp.element_size() + N * K + out.numel() * out.element_size() * (1 if residual is None else 2)))
     return out
@@ -953,11 +960,11 @@ def linear8_weight_grad(dy, x8, bias=True):
     _fits("linear8_weight_grad", N, K, T)
     if T == 0:
         return torch.zeros((N, K), dtype=torch.float32, device=dev), torch.zeros(N, dtype=torch.float32, device=dev) if bias else None
-    dw = torch.empty((N, K), dtype=torch.float32, device=dev)
-    db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
+    dw = dy.new_empty((N, K), dtype=torch.float32)
+    db = dy.new_empty(N, dtype=torch.float32) if bias else None
     need = _lib.lib().sdamd_linear8_weight_grad_ws_bytes(T, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _run8(dev, "sdamd_linear8_weight_grad", (_p(dy), _p(x8.q), _p(x8.scale), _p(dw), _p(db), _p(ws), need, T, N, K, _code8(x8.dtype)),
+    ws = dy.new_empty(need, dtype=torch.uint8) if need else None
+    _run8(dev, "sdamd_linear8_weight_grad", (dy.data_ptr(), x8.q.data_ptr(), x8.scale.data_ptr(), dw.data_ptr(), _p(db), _p(ws), need, T, N, K, _code8(x8.dtype)),
           lambda: ("linear8_weight_grad", 2.0 * T * N * K, f"T{T} N{N} K{K}", 2 * T * N + T * K + 4 * N * K))
     return dw, db
 
@@ -977,16 +984,15 @@ def layernorm_train(x, gamma, beta, eps=1e-5, out_dtype=None):
     rows = x.numel() // C
     _fits("layernorm_train", rows, C)
     if out_dtype in _FMT8:
-        y = _blocks8_empty(x.shape, out_dtype, dev)
+        y = _blocks8_empty(x, out_dtype)
         yp, sp, out_code, size = y.q, y.scale, _code8(out_dtype), 1
     else:
         out_code = _code(out_dtype)
-        y = torch.empty_like(x) if out_dtype == x.dtype else torch.empty(x.shape, dtype=out_dtype, device=dev)
+        y = torch.empty_like(x, dtype=out_dtype)
         yp, sp, size = y, None, y.element_size()
-    mean = torch.empty(rows, dtype=torch.float32, device=dev)
-    rstd = torch.empty_like(mean)
+    mean, rstd = gamma.new_empty(rows), gamma.new_empty(rows)
     if rows:
-        _run8(dev, "sdamd_layernorm_train", (_p(x), _p(yp), _p(sp), _p(gamma), _p(beta), _p(mean), _p(rstd), rows, C, float(eps), code, out_code),
+        _run8(dev, "sdamd_layernorm_train", (x.data_ptr(), yp.data_ptr(), _p(sp), gamma.data_ptr(), beta.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, C, float(eps), code, out_code),
               lambda: ("layernorm_train", x.numel() * (x.element_size() + size), f"rows{rows} C{C}", 0.0))
     return y, mean, rstd
 
@@ -1014,15 +1020,14 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
     if residual is not None:
         if not (residual.dtype == out_dtype and residual.is_contiguous() and residual.shape == dy.shape):
             raise _lib.SdamdError("layernorm_backward: residual %s %s has to be a contiguous %s %s" % (residual.dtype, tuple(residual.shape), out_dtype, tuple(dy.shape)))
-    dx = torch.empty_like(dy) if out_dtype == dy.dtype else torch.empty(dy.shape, dtype=out_dtype, device=dev)
+    dx = torch.empty_like(dy, dtype=out_dtype)
     if rows == 0:
         return dx, torch.zeros(C, dtype=torch.float32, device=dev), torch.zeros(C, dtype=torch.float32, device=dev)
-    dgamma = torch.empty(C, dtype=torch.float32, device=dev)
-    dbeta = torch.empty_like(dgamma)
+    dgamma, dbeta = gamma.new_empty(C), gamma.new_empty(C)
     need = _lib.lib().sdamd_layernorm_backward_ws_bytes(rows, C)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _run8(dev, "sdamd_layernorm_backward", (_p(dy), _p(x.q if is8 else x), _p(x.scale if is8 else None), _p(gamma), _p(mean), _p(rstd),
-                                            _p(residual), _p(dx), _p(dgamma), _p(dbeta), _p(ws), need, rows, C, dcode, xcode, ocode),
+    ws = dy.new_empty(need, dtype=torch.uint8) if need else None
+    _run8(dev, "sdamd_layernorm_backward", (dy.data_ptr(), (x.q if is8 else x).data_ptr(), x.scale.data_ptr() if is8 else 0, gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                                            _p(residual), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), _p(ws), need, rows, C, dcode, xcode, ocode),
           lambda: ("layernorm_backward", dy.numel() * (dy.element_size() + (1 if is8 else x.element_size()) +
                                                        dx.element_size() * (1 if residual is None else 2)), f"rows{rows} C{C}", 0.0))
     return dx, dgamma, dbeta
@@ -1037,11 +1042,11 @@ def geglu_train(h, dtype=torch.float8_e4m3fn):
         raise _lib.SdamdError("geglu_train: shape %s, strides %s" % (tuple(h.shape), tuple(h.stride())))
     Fh = h.shape[-1] // 2
     _fits("geglu_train", 2 * Fh)
-    out = torch.empty(h.shape[:-1] + (Fh,), dtype=h.dtype, device=dev)
-    kept = _blocks8_empty(h.shape, dtype, dev)
+    out = h.new_empty(h.shape[:-1] + (Fh,))
+    kept = _blocks8_empty(h, dtype)
     rows = kept.q.shape[0]
     if rows:
-        _run8(dev, "sdamd_geglu_train", (_p(h), _p(out), _p(kept.q), _p(kept.scale), rows, Fh, code, fmt),
+        _run8(dev, "sdamd_geglu_train", (h.data_ptr(), out.data_ptr(), kept.q.data_ptr(), kept.scale.data_ptr(), rows, Fh, code, fmt),
               lambda: ("geglu_train", h.numel() * (1.5 * h.element_size() + 1), f"rows{rows} F{Fh}", 0.0))
     return out, kept
 
@@ -1060,9 +1065,9 @@ def geglu_backward(dout, h, out_dtype=None):
     Fh = dout.shape[-1]
     rows = dout.numel() // Fh
     _fits("geglu_backward", 2 * Fh)
-    dh = torch.empty_like(h) if not is8 and h.dtype == out_dtype else torch.empty(h.shape, dtype=out_dtype, device=dev)
+    dh = dout.new_empty(h.shape, dtype=out_dtype)
     if rows:
-        _run8(dev, "sdamd_geglu_backward", (_p(dout), _p(h.q if is8 else h), _p(h.scale if is8 else None), _p(dh), rows, Fh, dcode, hcode, ocode),
+        _run8(dev, "sdamd_geglu_backward", (dout.data_ptr(), (h.q if is8 else h).data_ptr(), h.scale.data_ptr() if is8 else 0, dh.data_ptr(), rows, Fh, dcode, hcode, ocode),
               lambda: ("geglu_backward", dh.numel() * (dh.element_size() + (1 if is8 else h.element_size()) + dout.element_size() / 2),
                        f"rows{rows} F{Fh}", 0.0))
     return dh
