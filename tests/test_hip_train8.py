@@ -156,6 +156,23 @@ def test_quantize8_weight_is_exact(N, K, dtype):
     assert (b.q.view(torch.uint8)[:, K:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantize8_weight_takes_any_strides(dtype):
+    big = rnd(3, (300, 700), dtype)
+    big[7, 20], big[140, 300] = float("nan"), float("inf")
+    dev = big.to(DEV)
+    views = [lambda t: t[5:205, 3:604], lambda t: t[::2, ::3], lambda t: t[5:205, 3:604].t(), lambda t: t[::3, 1:300:2].t(),
+             lambda t: t[4:5, 9:400].expand(150, 391), lambda t: t[9:200, 4:5].expand(191, 140), lambda t: t[3:100, 5:10], lambda t: t[3:8, :300:7]]
+    for view in views:
+        a, b = ops.quantize8_weight(view(dev)), ops.quantize8_weight(view(dev).contiguous())
+        assert torch.equal(a.q.view(torch.uint8), b.q.view(torch.uint8)) and torch.equal(a.scale, b.scale)
+        plain = torch.where(view(big).isfinite(), view(big), torch.zeros((), dtype=dtype))
+        want, exps = blocks_ref(np64(plain), E4M3, 128)
+        assert np.array_equal(scales_of(a), exps)
+        got, fin = np64(a.dequantize(F32)), view(big).isfinite().numpy()
+        assert np.array_equal(got[fin], want[fin]) and np.isnan(got[~fin]).all()
+
+
 # ------------------------------------------------------------------ Linear
 def linear_ref(xq, wq, bias, res, act):
     v = xq @ wq.T
