@@ -138,20 +138,52 @@ __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ 
   if (sub == 0) { scale[(size_t)row * SP + fb] = (unsigned char)ev; scale[(size_t)row * SP + FB + fb] = (unsigned char)eg; }
   if (fb == (unsigned)FB - 1 && 2 * FB + sub < SP) scale[(size_t)row * SP + 2 * FB + sub] = 127;
 }
-// any F: a value's block and its gate's do not line up, so the blocks come from quant8_kernel and this pass gates
+// any F: a value's block and its gate's do not line up.  A workgroup quantises R whole rows, then gates them; it finds them in
+// the caches the second time.  (10000 x 1000 bf16: 22.5 us, as two launches 28.4; 65536 x
+// 960 107 and 138.  R with 32 blocks together; with 64 and 128 10000 x 1000 f32 takes 40.6 and 41.7 instead of 34.4.)
 template <typename T>
-__global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned nvec, int VR, int F) {
-  const unsigned i = blockIdx.x * 256u + threadIdx.x;
-  if (i >= nvec) return;
-  const unsigned row = i / (unsigned)VR;
-  const int c = (int)(i - row * (unsigned)VR) * 8;
-  const T* hr = h + (size_t)row * 2 * F;
-  float v[8], g[8], o[8];
-  row_load8(hr, c, F, v);
-  row_load8(hr + F, c, F, g);
+__global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned char* __restrict__ q,
+                                                         unsigned char* __restrict__ scale, long long rows, int R, int F, int KB, int SP, int fmt) {
+  const int t = threadIdx.x, sub = t & 15, VR = (F + 7) / 8;
+  const long long r0 = (long long)blockIdx.x * R;
+  const int n = (int)min((long long)R, rows - r0), blocks = n * KB, vecs = n * VR;
+  h += r0 * 2 * F;
+  out += r0 * F;
+  q += r0 * KB * B8_BLOCK;
+  scale += r0 * SP;
+  for (int b0 = t >> 4; b0 < blocks; b0 += 32) {           // two blocks requested at a time
+    Raw8<T> raw[2];
+    int row[2], kb[2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
-  row_store8(out + (size_t)row * F + c, F - c, o);
+    for (int u = 0; u < 2; ++u) {
+      const int b = min(b0 + 16 * u, blocks - 1);
+      row[u] = b / KB;
+      kb[u] = b - row[u] * KB;
+      raw[u] = raw8_load(h + (size_t)row[u] * 2 * F, kb[u] * B8_BLOCK + sub * 8, 2 * F);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float v[8];
+      raw8_get(raw[u], kb[u] * B8_BLOCK + sub * 8, 2 * F, v);
+      const int e = b8_exponent_of(b8_max16(b8_mag8(v)), fmt);
+      if (b0 + 16 * u < blocks) {
+        *reinterpret_cast<u32x2_t*>(q + ((size_t)row[u] * KB + kb[u]) * B8_BLOCK + sub * 8) = b8_pack8(v, e, fmt);
+        if (sub == 0) scale[(size_t)row[u] * SP + kb[u]] = (unsigned char)e;
+        if (kb[u] == KB - 1 && KB + sub < SP) scale[(size_t)row[u] * SP + KB + sub] = 127;
+      }
+    }
+  }
+  for (int i = t; i < vecs; i += 256) {
+    const int row = i / VR, c = (i - row * VR) * 8;
+    const T* hr = h + (size_t)row * 2 * F;
+    const Raw8<T> rv = raw8_load(hr, c, F), rg = raw8_load(hr + F, c, F);
+    float v[8], g[8], o[8];
+    raw8_get(rv, c, F, v);
+    raw8_get(rg, c, F, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
+    row_store8(out + (size_t)row * F + c, F - c, o);
+  }
 }
 
 // gelu(x) = x Phi(x) and its slope Phi(x) + x phi(x), erf as in gelu_erf_f (its exponential is phi's)
@@ -188,7 +220,20 @@ __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restric
       const u32x2_t qv = *reinterpret_cast<const u32x2_t*>(hr + c), qg = *reinterpret_cast<const u32x2_t*>(hr + F + c);
       b8_unpack8(qv, sr[c / B8_BLOCK], fmt, v);
       b8_unpack8(qg, sr[(F + c) / B8_BLOCK], fmt, g);
-    } else {                         // the gates start at any byte and may change block inside the vector
+    } else if (F > 8) {              // the gates start at any byte and may change block inside the vector
+      const int cc = min(c, F - 8), s = c - cc;                          // (read inside the row; its last, partial vector shifted down)
+      typedef unsigned long long __attribute__((aligned(1))) bytes8_t;
+      auto eight = [&](int at, float (&o)[8]) {
+        const unsigned long long b = *reinterpret_cast<const bytes8_t*>(hr + at + cc) >> s * 8;
+        b8_unpack8((u32x2_t){(unsigned)b, (unsigned)(b >> 32)}, 127, fmt, o);
+        const int from = at + c, to = B8_BLOCK - from % B8_BLOCK;        // (values to .. 7 are the next block's)
+        const float s0 = b8_scale(sr[from / B8_BLOCK]), s1 = b8_scale(sr[min(from + 7, 2 * F - 1) / B8_BLOCK]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] *= j < to ? s0 : s1;
+      };
+      eight(0, v);
+      eight(F, g);
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int cc = min(c + j, F - 1);
@@ -265,6 +310,7 @@ extern "C" int sdamd_dequant8(const void* q, const unsigned char* scale, void* o
   return 0;
 }
 
+static int geglu_rows_of_a_workgroup(int KB) { return max(1, 32 / KB); }
 template <typename T>
 static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned char* scale, long long rows, int F, int fmt, hipStream_t st) {
   const int SP = b8_scale_stride(2 * F);
@@ -273,17 +319,15 @@ static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned ch
     auto k = b8_past_cache((double)rows * F * sizeof(T)) ? geglu_train_kernel<T, true> : geglu_train_kernel<T, false>;
     k<<<(nblk + 15) / 16, 256, 0, st>>>(h, out, q, scale, nblk, F / B8_BLOCK, SP, fmt);
   } else {
-    const int KB = b8_kblocks(2 * F), VR = (F + 7) / 8;
-    const unsigned nblk = (unsigned)(rows * KB), nvec = (unsigned)(rows * VR);
-    quant8_kernel<T, 2><<<(nblk + 31) / 32, 256, 0, st>>>(h, q, scale, nblk, KB, 2 * F, 2 * F, SP, fmt);
-    geglu_rows_kernel<T><<<(nvec + 255) / 256, 256, 0, st>>>(h, out, nvec, VR, F);
+    const int KB = b8_kblocks(2 * F), R = geglu_rows_of_a_workgroup(KB);
+    geglu_rows_kernel<T><<<(unsigned)((rows + R - 1) / R), 256, 0, st>>>(h, out, q, scale, rows, R, F, KB, SP, fmt);
   }
 }
 
 extern "C" int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt, void* stream) {
   SD_CHECK(is_val(dtype) && is_fmt(fmt), "geglu_train: unsupported dtypes h=%d kept=%d", dtype, fmt);
   SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_train: bad shape rows=%lld F=%d", rows, F);
-  SD_CHECK(rows <= (1ll << 40) && rows * (long long)((F + 7) / 8) < (1ll << 31) && (F % B8_BLOCK == 0 || rows * (long long)b8_kblocks(2 * F) <= (1ll << 29) - 32),
+  SD_CHECK(rows <= (1ll << 40) && rows * (long long)((F + 7) / 8) < (1ll << 31) && (F % B8_BLOCK == 0 || rows / geglu_rows_of_a_workgroup(b8_kblocks(2 * F)) < (1ll << 24) - 1),
            "geglu_train: too large, rows=%lld F=%d", rows, F);
   if (dtype == SDAMD_BF16) geglu_train_launch<bf16_t>((const bf16_t*)h, (bf16_t*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
   else geglu_train_launch<float>((const float*)h, (float*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);

@@ -1035,7 +1035,7 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
 
 def geglu_train(h, dtype=torch.float8_e4m3fn):
     """GeGLU that keeps its input in 8 bits: h [..., 2F] (value | gate) -> (value * gelu(gate) [..., F] in h's type, Blocks8
-    of h), in one pass over h where F is a multiple of 128."""
+    of h), in one pass over h."""
     fmt, code = _code8(dtype), _code(h.dtype)
     dev = _dev8("geglu_train", h)
     if not (h.dim() >= 1 and h.is_contiguous() and h.shape[-1] > 0 and h.shape[-1] % 2 == 0):
