@@ -52,6 +52,7 @@ template <int FMT> __device__ __forceinline__ void w8_to_bf16(u32x4_t v, float s
 __device__ __forceinline__ int w8_swz(int t) { return (t & 3) | (((t >> 3) & 1) << 2); }
 
 // DMA: rows of dy are 16-byte aligned (N % 8 == 0 and an aligned base) and go straight to LDS; otherwise through registers
+// (8192 x 1280 x 1280: 49.7 us; 1284 columns, through registers: 66.8)
 template <int BT_N, int BT_K, int WGN, int WGK, int FMT, bool DMA>
 __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
   constexpr int NT = 64 * WGN * WGK, TN = BT_N / WGN / 16, TK = BT_K / WGK / 16;
@@ -146,9 +147,13 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
 #pragma unroll
       for (int i = 0; i < DI; ++i) {
         const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-        float v[8];
-        raw8_get(rd[DMA ? 0 : i], n0 + c * 8, p.N, v);
-        u32x4_t o = {pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
+        u32x4_t o = rd[DMA ? 0 : i].a;
+        const int s = p.N < 8 ? 0 : max(n0 + c * 8 - (p.N - 8), 0);      // a row's last, partial piece was read s columns early
+        if (s > 0) {
+          if (s & 4) o = (u32x4_t){o[2], o[3], 0u, 0u};
+          if (s & 2) o = (u32x4_t){o[1], o[2], o[3], 0u};
+          if (s & 1) o = (u32x4_t){o[0] >> 16 | o[1] << 16, o[1] >> 16 | o[2] << 16, o[2] >> 16 | o[3] << 16, o[3] >> 16};
+        }
         if (t >= left) o = (u32x4_t){0u, 0u, 0u, 0u};
         *reinterpret_cast<u32x4_t*>(smem + buf * STAGE + t * ROWN + (((c >> 1) ^ w8_swz(t)) * 2 + (c & 1)) * 16) = o;
       }
