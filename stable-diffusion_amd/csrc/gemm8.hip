@@ -531,16 +531,17 @@ __global__ __launch_bounds__(64 * g8_rows_waves<MT>()) void gemm8_rows_kernel(G8
 // Few tiles: the rows kernel, which splits K over the waves of a workgroup and gives every 16 columns a workgroup; the tile
 // kernel's time is then the length of its walk over K (0.65 us a step, 1.3 us in its f32 form) whatever the tiles.  Its time
 // and the tile kernel's, us: 256 x 1280 -> 1280 (20 tiles) 5.0 and 9.2; 512 x 5120 -> 1280 (40) 15.9 and 32.5; 2048 x 320 -> 320
-// (48) 4.8 and 6.1; 1024 x 1280 -> 1280 (80) 10.4 and 9.6; 2048 x 640 -> 640 (80) 8.1 and 6.5.  f32: 2048 x 640 -> 640 9.0 and
+// (48) 4.8 and 6.1; 1024 x 1280 -> 1280 (80) 10.4 and 9.6; 2048 x 640 -> 640 (80) 8.1 and 6.5, but
+// with a long K 1024 x 5120 -> 1280 (80) 28.9 and 37.6, 4096 x 2560 -> 320 (96) 19.6 and 20.9.  f32: 2048 x 640 -> 640 9.0 and
 // 10.2; 1024 x 1280 -> 1280 12.5 and 16.6; 4096 x 320 -> 320 (96) 7.7 and 8.2; 512 x 1280 -> 5120 (160) 22.4 and 17.9.
 static long long g8_tiles(int M, int N, int b) { return (long long)((M + b - 1) / b) * ((N + b - 1) / b); }
 constexpr int G8_MAX_WIDTH = 1 << 24;
 // (Both planned from one sample's rows under sdamd_set_plan_samples: they decide the order of the sums.  The tile kernel's
 // forms give the same bits.)
 static int g8_row_tiles(int rows) { const int M = plan_rows(rows); return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
-static bool g8_few_rows(int rows, int N, bool exact) {
+static bool g8_few_rows(int rows, int N, int K, bool exact) {
   const int M = plan_rows(rows);
-  return M <= 64 || g8_tiles(M, N, 128) < (exact ? 128 : 64);
+  return M <= 64 || g8_tiles(M, N, 128) < (exact ? 128 : b8_kblocks(K) > 16 ? 96 : 64);
 }
 // That kernel can quantise rows on its way.  A wave then quantises its blocks of K for all the workgroup's 16-row tiles,
 // every 16 columns anew: no second launch and no buffers for the blocks, half the time of an eager call (64 x 320 -> 1280: 8.7
@@ -552,7 +553,7 @@ extern "C" int sdamd_linear8_quantises(int M, int N, int K, int out_dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const int tiles = g8_row_tiles(M), waves = tiles == 4 ? 8 : 16;
   const long long groups = (long long)((M + 16 * tiles - 1) / (16 * tiles)) * ((N + 15) / 16);
-  return g8_few_rows(M, N, out_dtype == SDAMD_F32) && (b8_kblocks(K) + waves - 1) / waves * tiles * ((groups + 255) / 256) <= 4;
+  return g8_few_rows(M, N, K, out_dtype == SDAMD_F32) && (b8_kblocks(K) + waves - 1) / waves * tiles * ((groups + 255) / 256) <= 4;
 }
 
 template <int BM, int BN, int WGM, int WGN, int PLACES, int FMT, bool EXACT, typename TO>
@@ -592,7 +593,7 @@ static int g8_rows_launch(G8Args p, hipStream_t st) {
 
 template <int FMT, bool EXACT, typename TO>
 static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
-  if (g8_few_rows(p.M, p.N, EXACT)) {
+  if (g8_few_rows(p.M, p.N, p.K, EXACT)) {
     const int mt = g8_row_tiles(p.M);
 #define G8_ROWS(TX)                                                                              \
   (mt == 1 ? g8_rows_launch<1, FMT, EXACT, TO, TX>(p, st)                                  \
