@@ -286,9 +286,10 @@ int sdamd_layernorm_backward(const void* dy, const void* x, const unsigned char*
                              const float* mean, const float* rstd, const void* residual, void* dx, float* dgamma,
                              float* dbeta, void* ws, size_t ws_bytes, int rows, int C, int dy_dtype, int x_dtype,
                              int dx_dtype, void* stream);
-/* h [rows][2F] (value | gate) -> out [rows][F] = value * gelu_erf(gate) and h's row blocks (fmt) */
-int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt,
-                      void* stream);
+/* h [rows][2F] (value | gate) -> out [rows][F] = value * gelu_erf(gate), of h's dtype or row blocks with out_scale (out_dtype
+ * SDAMD_E4M3 / SDAMD_E5M2; out_scale null otherwise), and h's row blocks (fmt) */
+int sdamd_geglu_train(const void* h, void* out, unsigned char* out_scale, void* q, unsigned char* scale, long long rows, int F,
+                      int dtype, int out_dtype, int fmt, void* stream);
 /* dh [rows][2F] = (dout gelu(gate) | dout value gelu'(gate)); h: F32 / BF16, or row blocks with h_scale */
 int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, long long rows, int F,
                          int dout_dtype, int h_dtype, int dh_dtype, void* stream);

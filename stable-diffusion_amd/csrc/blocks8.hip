@@ -114,12 +114,15 @@ __global__ __launch_bounds__(256) void dequant8_kernel(const unsigned char* __re
   row_store8(out + (size_t)row * K + c, K - c, v);
 }
 
-// ---- GeGLU that keeps its input in 8 bits: h [rows][2F] -> out [rows][F] = value * gelu(gate), and h's blocks.
-// 65536 x 1280 bf16: 119 us = 5.6 TB/s.
+// ---- GeGLU that keeps its input in 8 bits: h [rows][2F] -> out [rows][F] = value * gelu(gate), of h's type or as blocks of
+// another Linear's operand, and h's blocks.
+// 65536 x 1280 bf16: 114 us = 5.9 TB/s; into blocks 112, where a quantiser behind it makes 170.
 // F % 128 == 0: the 16 lanes that hold a value block hold the gate block of the same columns too, so h is read once.
-template <typename T, bool PAST>
-__global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned char* __restrict__ q,
-                                                          unsigned char* __restrict__ scale, unsigned nblk, int FB, int SP, int fmt) {
+enum GegluOut { GEGLU_DENSE, GEGLU_PAST, GEGLU_BLOCKS };    // PAST: past the cache (b8_past_cache)
+template <typename T, GegluOut OUT>
+__global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ h, void* __restrict__ out, unsigned char* __restrict__ out_scale,
+                                                          unsigned char* __restrict__ q, unsigned char* __restrict__ scale, unsigned nblk, int FB,
+                                                          int SP, int fmt, int out_fmt) {
   const int sub = threadIdx.x & 15;
   const unsigned b = blockIdx.x * 16u + (threadIdx.x >> 4);
   const unsigned bb = min(b, nblk - 1), row = bb / (unsigned)FB, fb = bb - row * (unsigned)FB;
@@ -129,10 +132,18 @@ __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ 
   raw8_get(rv, sub * 8, B8_BLOCK, v);
   raw8_get(rg, sub * 8, B8_BLOCK, g);
   const int ev = b8_exponent_of(b8_max16(b8_mag8(v)), fmt), eg = b8_exponent_of(b8_max16(b8_mag8(g)), fmt);
-  if (b >= nblk) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
-  row_store8<PAST>(out + (size_t)bb * B8_BLOCK + sub * 8, 8, o);
+  const int eo = OUT == GEGLU_BLOCKS ? b8_exponent_of(b8_max16(b8_mag8(o)), out_fmt) : 0;
+  if (b >= nblk) return;
+  if constexpr (OUT == GEGLU_BLOCKS) {
+    const int SO = (FB + 3) / 4 * 4;
+    *reinterpret_cast<u32x2_t*>((unsigned char*)out + (size_t)bb * B8_BLOCK + sub * 8) = b8_pack8(o, eo, out_fmt);
+    if (sub == 0) out_scale[(size_t)row * SO + fb] = (unsigned char)eo;
+    if (fb == (unsigned)FB - 1 && FB + sub < SO) out_scale[(size_t)row * SO + FB + sub] = 127;
+  } else {
+    row_store8<OUT == GEGLU_PAST>((T*)out + (size_t)bb * B8_BLOCK + sub * 8, 8, o);
+  }
   *reinterpret_cast<u32x2_t*>(q + vb * B8_BLOCK + sub * 8) = b8_pack8(v, ev, fmt);
   *reinterpret_cast<u32x2_t*>(q + gb * B8_BLOCK + sub * 8) = b8_pack8(g, eg, fmt);
   if (sub == 0) { scale[(size_t)row * SP + fb] = (unsigned char)ev; scale[(size_t)row * SP + FB + fb] = (unsigned char)eg; }
@@ -141,14 +152,14 @@ __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ 
 // any F: a value's block and its gate's do not line up.  A workgroup quantises R whole rows, then gates them; it finds them in
 // the caches the second time.  (10000 x 1000 bf16: 22.5 us, as two launches 28.4; 65536 x
 // 960 107 and 138.  R with 32 blocks together; with 64 and 128 10000 x 1000 f32 takes 40.6 and 41.7 instead of 34.4.)
-template <typename T>
-__global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h, T* __restrict__ out, unsigned char* __restrict__ q,
-                                                         unsigned char* __restrict__ scale, long long rows, int R, int F, int KB, int SP, int fmt) {
+template <typename T, bool BLOCKS>
+__global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h, void* __restrict__ out, unsigned char* __restrict__ out_scale,
+                                                         unsigned char* __restrict__ q, unsigned char* __restrict__ scale, long long rows, int R,
+                                                         int F, int KB, int SP, int fmt, int out_fmt) {
   const int t = threadIdx.x, sub = t & 15, VR = (F + 7) / 8;
   const long long r0 = (long long)blockIdx.x * R;
   const int n = (int)min((long long)R, rows - r0), blocks = n * KB, vecs = n * VR;
   h += r0 * 2 * F;
-  out += r0 * F;
   q += r0 * KB * B8_BLOCK;
   scale += r0 * SP;
   for (int b0 = t >> 4; b0 < blocks; b0 += 32) {           // two blocks requested at a time
@@ -173,16 +184,33 @@ __global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h
       }
     }
   }
-  for (int i = t; i < vecs; i += 256) {
-    const int row = i / VR, c = (i - row * VR) * 8;
+  auto gate = [&](int row, int c, float (&o)[8]) {
     const T* hr = h + (size_t)row * 2 * F;
     const Raw8<T> rv = raw8_load(hr, c, F), rg = raw8_load(hr + F, c, F);
-    float v[8], g[8], o[8];
+    float v[8], g[8];
     raw8_get(rv, c, F, v);
     raw8_get(rg, c, F, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);
-    row_store8(out + (size_t)row * F + c, F - c, o);
+    for (int j = 0; j < 8; ++j) o[j] = v[j] * gelu_erf_f(g[j]);          // (zeros past F)
+  };
+  if constexpr (BLOCKS) {
+    const int KO = (F + B8_BLOCK - 1) / B8_BLOCK, SO = (KO + 3) / 4 * 4;
+    for (int b = t >> 4; b < n * KO; b += 16) {
+      const int row = b / KO, kb = b - row * KO;
+      float o[8];
+      gate(row, kb * B8_BLOCK + sub * 8, o);
+      const int e = b8_exponent_of(b8_max16(b8_mag8(o)), out_fmt);
+      *reinterpret_cast<u32x2_t*>((unsigned char*)out + ((size_t)(r0 + row) * KO + kb) * B8_BLOCK + sub * 8) = b8_pack8(o, e, out_fmt);
+      if (sub == 0) out_scale[(size_t)(r0 + row) * SO + kb] = (unsigned char)e;
+      if (kb == KO - 1 && KO + sub < SO) out_scale[(size_t)(r0 + row) * SO + KO + sub] = 127;
+    }
+  } else {
+    for (int i = t; i < vecs; i += 256) {
+      const int row = i / VR, c = (i - row * VR) * 8;
+      float o[8];
+      gate(row, c, o);
+      row_store8((T*)out + (size_t)(r0 + row) * F + c, F - c, o);
+    }
   }
 }
 
@@ -312,25 +340,30 @@ extern "C" int sdamd_dequant8(const void* q, const unsigned char* scale, void* o
 
 static int geglu_rows_of_a_workgroup(int KB) { return max(1, 32 / KB); }
 template <typename T>
-static void geglu_train_launch(const T* h, T* out, unsigned char* q, unsigned char* scale, long long rows, int F, int fmt, hipStream_t st) {
+static void geglu_train_launch(const T* h, void* out, unsigned char* out_scale, unsigned char* q, unsigned char* scale, long long rows, int F,
+                               int fmt, int out_dtype, hipStream_t st) {
   const int SP = b8_scale_stride(2 * F);
   if (F % B8_BLOCK == 0) {
     const unsigned nblk = (unsigned)(rows * (F / B8_BLOCK));
-    auto k = b8_past_cache((double)rows * F * sizeof(T)) ? geglu_train_kernel<T, true> : geglu_train_kernel<T, false>;
-    k<<<(nblk + 15) / 16, 256, 0, st>>>(h, out, q, scale, nblk, F / B8_BLOCK, SP, fmt);
+    auto k = is_fmt(out_dtype) ? geglu_train_kernel<T, GEGLU_BLOCKS>
+             : b8_past_cache((double)rows * F * sizeof(T)) ? geglu_train_kernel<T, GEGLU_PAST> : geglu_train_kernel<T, GEGLU_DENSE>;
+    k<<<(nblk + 15) / 16, 256, 0, st>>>(h, out, out_scale, q, scale, nblk, F / B8_BLOCK, SP, fmt, out_dtype);
   } else {
     const int KB = b8_kblocks(2 * F), R = geglu_rows_of_a_workgroup(KB);
-    geglu_rows_kernel<T><<<(unsigned)((rows + R - 1) / R), 256, 0, st>>>(h, out, q, scale, rows, R, F, KB, SP, fmt);
+    auto k = is_fmt(out_dtype) ? geglu_rows_kernel<T, true> : geglu_rows_kernel<T, false>;
+    k<<<(unsigned)((rows + R - 1) / R), 256, 0, st>>>(h, out, out_scale, q, scale, rows, R, F, KB, SP, fmt, out_dtype);
   }
 }
 
-extern "C" int sdamd_geglu_train(const void* h, void* out, void* q, unsigned char* scale, long long rows, int F, int dtype, int fmt, void* stream) {
-  SD_CHECK(is_val(dtype) && is_fmt(fmt), "geglu_train: unsupported dtypes h=%d kept=%d", dtype, fmt);
+extern "C" int sdamd_geglu_train(const void* h, void* out, unsigned char* out_scale, void* q, unsigned char* scale, long long rows, int F, int dtype,
+                                 int out_dtype, int fmt, void* stream) {
+  SD_CHECK(is_val(dtype) && (out_dtype == dtype || is_fmt(out_dtype)) && is_fmt(fmt), "geglu_train: unsupported dtypes h=%d out=%d kept=%d", dtype, out_dtype, fmt);
+  SD_CHECK(!is_fmt(out_dtype) || out_scale, "geglu_train: 8-bit output without room for its scales");
   SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_train: bad shape rows=%lld F=%d", rows, F);
   SD_CHECK(rows <= (1ll << 40) && rows * (long long)((F + 7) / 8) < (1ll << 31) && (F % B8_BLOCK == 0 || rows / geglu_rows_of_a_workgroup(b8_kblocks(2 * F)) < (1ll << 24) - 1),
            "geglu_train: too large, rows=%lld F=%d", rows, F);
-  if (dtype == SDAMD_BF16) geglu_train_launch<bf16_t>((const bf16_t*)h, (bf16_t*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
-  else geglu_train_launch<float>((const float*)h, (float*)out, (unsigned char*)q, scale, rows, F, fmt, (hipStream_t)stream);
+  if (dtype == SDAMD_BF16) geglu_train_launch<bf16_t>((const bf16_t*)h, out, out_scale, (unsigned char*)q, scale, rows, F, fmt, out_dtype, (hipStream_t)stream);
+  else geglu_train_launch<float>((const float*)h, out, out_scale, (unsigned char*)q, scale, rows, F, fmt, out_dtype, (hipStream_t)stream);
   SD_LAUNCH_CHECK("geglu_train");
   return 0;
 }

@@ -843,11 +843,10 @@ class Blocks8:
         return out
 
 
-def _blocks8_empty(x, dtype):
-    """Uninitialised blocks of x's shape for the kernels to fill."""
-    shape = tuple(x.shape)
-    K = shape[-1]
-    rows, kb = x.numel() // K, -(-K // BLOCK8)
+def _blocks8_empty(x, dtype, shape=None):
+    """Uninitialised blocks of x's shape (or ``shape``, of as many rows) for the kernels to fill."""
+    rows, shape = x.numel() // x.shape[-1], tuple(shape or x.shape)
+    kb = -(-shape[-1] // BLOCK8)
     b = Blocks8.__new__(Blocks8)
     b.q = x.new_empty((rows, kb * BLOCK8), dtype=dtype)
     b.scale = x.new_empty((rows, -(-kb // 4) * 4), dtype=torch.uint8)
@@ -1033,21 +1032,28 @@ def layernorm_backward(dy, x, gamma, mean, rstd, residual=None, out_dtype=None):
     return dx, dgamma, dbeta
 
 
-def geglu_train(h, dtype=torch.float8_e4m3fn):
-    """GeGLU that keeps its input in 8 bits: h [..., 2F] (value | gate) -> (value * gelu(gate) [..., F] in h's type, Blocks8
-    of h), in one pass over h."""
+def geglu_train(h, dtype=torch.float8_e4m3fn, out_dtype=None):
+    """GeGLU that keeps its input in 8 bits: h [..., 2F] (value | gate) -> (value * gelu(gate) [..., F], Blocks8 of h in
+    ``dtype``), in one pass over h.  ``out_dtype``: h's type (default), or float8_e4m3fn / float8_e5m2 -- then the product is
+    Blocks8, the operand of the following ``linear8`` and its checkpoint, rounded once, from float32."""
     fmt, code = _code8(dtype), _code(h.dtype)
     dev = _dev8("geglu_train", h)
     if not (h.dim() >= 1 and h.is_contiguous() and h.shape[-1] > 0 and h.shape[-1] % 2 == 0):
         raise _lib.SdamdError("geglu_train: shape %s, strides %s" % (tuple(h.shape), tuple(h.stride())))
     Fh = h.shape[-1] // 2
     _fits("geglu_train", 2 * Fh)
-    out = h.new_empty(h.shape[:-1] + (Fh,))
     kept = _blocks8_empty(h, dtype)
     rows = kept.q.shape[0]
+    if out_dtype is None or out_dtype == h.dtype:
+        out = op = h.new_empty(h.shape[:-1] + (Fh,))
+        sp, out_code = None, code
+    else:
+        out_code = _code8(out_dtype)
+        out = _blocks8_empty(h, out_dtype, h.shape[:-1] + (Fh,))
+        op, sp = out.q, out.scale
     if rows:
-        _run8(dev, "sdamd_geglu_train", (h.data_ptr(), out.data_ptr(), kept.q.data_ptr(), kept.scale.data_ptr(), rows, Fh, code, fmt),
-              lambda: ("geglu_train", h.numel() * (1.5 * h.element_size() + 1), f"rows{rows} F{Fh}", 0.0))
+        _run8(dev, "sdamd_geglu_train", (h.data_ptr(), op.data_ptr(), _p(sp), kept.q.data_ptr(), kept.scale.data_ptr(), rows, Fh, code, out_code, fmt),
+              lambda: ("geglu_train", h.numel() * (h.element_size() + 0.5 * op.element_size() + 1), f"rows{rows} F{Fh}", 0.0))
     return out, kept
 
 

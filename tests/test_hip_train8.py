@@ -594,6 +594,30 @@ def test_geglu_train_and_backward(rows, F, dtype, fmt):
         assert torch.equal(mixed, ops.geglu_backward(dout.to(DEV), kept).to(BF16))
 
 
+@pytest.mark.parametrize("rows,F", [(1, 1), (3, 7), (2, 64), (5, 100), (9, 128), (4, 129), (33, 320), (6, 1280), (3, 515), (70, 384)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+def test_geglu_train_into_blocks(rows, F, dtype, fmt):
+    h = rnd(rows + F, (rows, 2 * F), dtype, 1.5)
+    dense, kept = ops.geglu_train(h.to(DEV))
+    out, kept2 = ops.geglu_train(h.to(DEV), out_dtype=fmt)
+    assert out.shape == (rows, F) and out.dtype == fmt and out.block_rows == 1
+    assert torch.equal(kept.q.view(torch.uint8), kept2.q.view(torch.uint8)) and torch.equal(kept.scale, kept2.scale)
+    assert (out.q.view(torch.uint8)[:, F:] == 0).all()
+    if dtype == F32:                                 # the same float32 products, quantised here or afterwards
+        two = ops.quantize8(dense, fmt)
+        assert torch.equal(out.q.view(torch.uint8), two.q.view(torch.uint8)) and torch.equal(out.scale, two.scale)
+    H = np64(h)
+    want, _, _ = geglu_ref(H[:, :F], H[:, F:])
+    off = 4e-7 * np.abs(H[:, :F] * H[:, F:]) + 4 * U * np.abs(want)        # of the product itself, as above
+    scale = np.repeat(2.0 ** scales_of(out), 128, 1)[:, :F]
+    half, low, top = (2.0 ** -4, 2.0 ** -10, 448.0) if fmt == E4M3 else (2.0 ** -3, 2.0 ** -17, 57344.0)     # half a step: relative, and of the smallest numbers
+    close(np64(out.dequantize(F32)), want, off + half * (np.abs(want) + off) + low * scale, "blocks")
+    for b in range(-(-F // 128)):                    # the smallest scale that the product, as exact as it is, fits
+        part, slack, s = np.abs(want[:, b * 128:b * 128 + 128]), off[:, b * 128:b * 128 + 128], scale[:, b * 128]
+        assert ((part - slack).max(1) <= top * s).all() and ((part + slack).max(1) > top * s / 2).all()
+
+
 def test_geglu_gradient_against_differences():
     rows, F, step = 3, 50, 1e-5
     h, dout = rnd(1, (rows, 2 * F)), rnd(2, (rows, F))
@@ -613,6 +637,10 @@ def test_geglu_refusals_and_empty():
             bad()
     with pytest.raises(TypeError):
         ops.geglu_backward(d.half(), h)
+    for bad in (BF16, torch.float16, torch.int8):
+        with pytest.raises(TypeError):
+            ops.geglu_train(h, out_dtype=bad)
+    assert ops.geglu_train(torch.empty(0, 64, device=DEV), out_dtype=E4M3)[0].shape == (0, 32)
     out, kept = ops.geglu_train(torch.empty(0, 64, device=DEV))
     assert out.shape == (0, 32) and ops.geglu_backward(torch.empty(0, 32, device=DEV), kept).shape == (0, 64)
 

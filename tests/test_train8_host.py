@@ -37,7 +37,7 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_linear8_weight_grad(P, P + 4, P, P, P, 0, 0, 4, 4, 4, 2, 0), "aligned")
     refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 1 << 24, 768, 1e-5, 0, 0, 0), "too many rows")
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, 1 << 30, 1 << 29, 8, 0, 0, 0, 0), "too many rows")
-    refused(L.sdamd_geglu_train(P, P, P, P, 1 << 40, 64, 0, 2, 0), "too large")
+    refused(L.sdamd_geglu_train(P, P, 0, P, P, 1 << 40, 64, 0, 0, 2, 0), "too large")
     refused(L.sdamd_geglu_backward(P, P, 0, P, 1 << 40, 64, 0, 0, 0, 0), "too large")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 0, 4, 4, 2, 0), "bad shape")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, 4, 4, 1, 0), "unsupported dtype")
@@ -53,8 +53,10 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, many - 1, 4096, 64, 0, 0, 0, 0), "workspace")
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need, 4, 64, 0, 2, 0, 0), "without its scales")
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, need, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
-    refused(L.sdamd_geglu_train(P, P, P, P, 0, 64, 0, 2, 0), "bad shape")
-    refused(L.sdamd_geglu_train(P, P, P, P, 4, 64, 2, 2, 0), "unsupported dtypes")
+    refused(L.sdamd_geglu_train(P, P, 0, P, P, 0, 64, 0, 0, 2, 0), "bad shape")
+    refused(L.sdamd_geglu_train(P, P, 0, P, P, 4, 64, 2, 2, 2, 0), "unsupported dtypes")
+    refused(L.sdamd_geglu_train(P, P, 0, P, P, 4, 64, 1, 0, 2, 0), "unsupported dtypes")
+    refused(L.sdamd_geglu_train(P, P, 0, P, P, 4, 64, 0, 2, 2, 0), "without room")
     refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 0, 2, 0, 0), "without its scales")
     refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
 
@@ -62,8 +64,8 @@ def test_c_boundary_refuses_bad_arguments():
 def test_c_boundary_keeps_launches_below_2_to_32_threads():
     refused(L.sdamd_quant8(P, P, P, (1 << 29) - 31, 8, 8, 0, 2, 0), "too large")
     refused(L.sdamd_dequant8(P, P, P, (1 << 28) - 15, 8, 1, 2, 0, 0), "too large")
-    refused(L.sdamd_geglu_train(P, P, P, P, 1 << 30, 4, 0, 2, 0), "too large")
-    refused(L.sdamd_geglu_train(P, P, P, P, 1 << 30, 128, 0, 2, 0), "too large")
+    refused(L.sdamd_geglu_train(P, P, 0, P, P, 1 << 30, 4, 0, 0, 2, 0), "too large")
+    refused(L.sdamd_geglu_train(P, P, P, P, P, 1 << 30, 128, 0, 3, 2, 0), "too large")
     refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, (1 << 27) - 31, 512, 1e-5, 0, 0, 0), "too many rows")
 
 
