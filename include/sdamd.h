@@ -290,9 +290,10 @@ int sdamd_layernorm_backward(const void* dy, const void* x, const unsigned char*
  * SDAMD_E4M3 / SDAMD_E5M2; out_scale null otherwise), and h's row blocks (fmt) */
 int sdamd_geglu_train(const void* h, void* out, unsigned char* out_scale, void* q, unsigned char* scale, long long rows, int F,
                       int dtype, int out_dtype, int fmt, void* stream);
-/* dh [rows][2F] = (dout gelu(gate) | dout value gelu'(gate)); h: F32 / BF16, or row blocks with h_scale */
-int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, long long rows, int F,
-                         int dout_dtype, int h_dtype, int dh_dtype, void* stream);
+/* dh [rows][2F] = (dout gelu(gate) | dout value gelu'(gate)); h: F32 / BF16, or row blocks with h_scale.  q (may be null):
+ * dh's row blocks too, of type q_fmt with q_scale, for bf16 dh and F % 128 == 0 */
+int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, void* q, unsigned char* q_scale,
+                         long long rows, int F, int dout_dtype, int h_dtype, int dh_dtype, int q_fmt, void* stream);
 
 #ifdef __cplusplus
 }

@@ -66,7 +66,7 @@ SIGNATURES = {
     "sdamd_layernorm_backward_ws_bytes": (_sz, [_i, _i]),
     "sdamd_layernorm_backward": (_i, [_vp] * 11 + [_sz] + [_i] * 5 + [_vp]),
     "sdamd_geglu_train": (_i, [_vp] * 5 + [_ll, _i, _i, _i, _i, _vp]),
-    "sdamd_geglu_backward": (_i, [_vp] * 4 + [_ll, _i, _i, _i, _i, _vp]),
+    "sdamd_geglu_backward": (_i, [_vp] * 6 + [_ll, _i, _i, _i, _i, _i, _vp]),
 }
 
 _lib = None

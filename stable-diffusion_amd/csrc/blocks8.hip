@@ -230,13 +230,16 @@ __device__ __forceinline__ void gelu_slope(float x, float& gelu, float& slope) {
 }
 
 // ---- GeGLU backward: dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
-// (TH = unsigned char).  65536 x 1280 bf16 from e4m3: 130 us = 5.2 TB/s.
-template <typename TD, typename TH, typename TO, bool PAST>
+// (TH = unsigned char).  BLOCKS (F % 128 == 0, dh bf16): dh's blocks too, of the values as dh holds them, the operand of the Linear that
+// takes it on.  65536 x 1280 bf16 from e4m3: 128 us = 5.2 TB/s; with blocks 160, where a quantiser behind it
+// makes 219.
+template <typename TD, typename TH, typename TO, bool PAST, bool BLOCKS>
 __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restrict__ dout, const TH* __restrict__ h,
                                                              const unsigned char* __restrict__ scale, TO* __restrict__ dh,
-                                                             unsigned nvec, int VR, int F, int ldh, int SP, int fmt) {
+                                                             unsigned nvec, int VR, int F, int ldh, int SP, int fmt,
+                                                             unsigned char* __restrict__ q, unsigned char* __restrict__ q_scale, int q_fmt) {
   const unsigned i = blockIdx.x * 256u + threadIdx.x;
-  if (i >= nvec) return;
+  if (i >= nvec) return;                         // (BLOCKS: in whole groups of 16)
   const unsigned row = i / (unsigned)VR;
   const int c = (int)(i - row * (unsigned)VR) * 8;
   const TH* hr = h + (size_t)row * ldh;
@@ -283,6 +286,19 @@ __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restric
   }
   row_store8<PAST>(dh + (size_t)row * 2 * F + c, F - c, dv);
   row_store8<PAST>(dh + (size_t)row * 2 * F + F + c, F - c, dg);
+  if constexpr (BLOCKS) {
+    const int sub = threadIdx.x & 15, FB = F / B8_BLOCK, fb = c / B8_BLOCK;
+    auto block = [&](float (&x)[8], int col) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = bf2f(f2bf(x[j]));
+      const int e = b8_exponent_of(b8_max16(b8_mag8(x)), q_fmt);
+      *reinterpret_cast<u32x2_t*>(q + (size_t)row * 2 * F + col) = b8_pack8(x, e, q_fmt);
+      if (sub == 0) q_scale[(size_t)row * SP + col / B8_BLOCK] = (unsigned char)e;
+    };
+    block(dv, c);
+    block(dg, F + c);
+    if (fb == FB - 1 && 2 * FB + sub < SP) q_scale[(size_t)row * SP + 2 * FB + sub] = 127;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -368,11 +384,21 @@ extern "C" int sdamd_geglu_train(const void* h, void* out, unsigned char* out_sc
   return 0;
 }
 
-extern "C" int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, long long rows, int F,
-                                    int dout_dtype, int h_dtype, int dh_dtype, void* stream) {
+template <typename TD, typename TH, typename TO, typename... A>
+static void geglu_backward_launch(dim3 grid, hipStream_t st, bool past, bool blocks, A... a) {
+  auto k = past ? geglu_backward_kernel<TD, TH, TO, true, false> : geglu_backward_kernel<TD, TH, TO, false, false>;
+  if constexpr (sizeof(TO) == 2) {
+    if (blocks) k = past ? geglu_backward_kernel<TD, TH, TO, true, true> : geglu_backward_kernel<TD, TH, TO, false, true>;
+  }
+  k<<<grid, 256, 0, st>>>(a...);
+}
+
+extern "C" int sdamd_geglu_backward(const void* dout, const void* h, const unsigned char* h_scale, void* dh, void* q, unsigned char* q_scale,
+                                    long long rows, int F, int dout_dtype, int h_dtype, int dh_dtype, int q_fmt, void* stream) {
   SD_CHECK(is_val(dout_dtype) && is_val(dh_dtype) && (is_val(h_dtype) || is_fmt(h_dtype)), "geglu_backward: unsupported dtypes dout=%d h=%d dh=%d",
            dout_dtype, h_dtype, dh_dtype);
   SD_CHECK(!is_fmt(h_dtype) || h_scale, "geglu_backward: 8-bit h without its scales");
+  SD_CHECK(!q || (is_fmt(q_fmt) && q_scale && dh_dtype == SDAMD_BF16 && F % B8_BLOCK == 0), "geglu_backward: blocks of dh need room for scales, bf16 dh and F %% 128 == 0 (F=%d)", F);
   SD_CHECK(rows > 0 && F > 0 && F <= (1 << 29), "geglu_backward: bad shape rows=%lld F=%d", rows, F);
   const int VR = (F + 7) / 8;
   SD_CHECK(rows <= (1ll << 40) && rows * (long long)VR < (1ll << 31), "geglu_backward: too large, rows=%lld F=%d", rows, F);
@@ -381,8 +407,8 @@ extern "C" int sdamd_geglu_backward(const void* dout, const void* h, const unsig
   const int SP = b8_scale_stride(2 * F), ldq = b8_kblocks(2 * F) * B8_BLOCK;
   const bool past = b8_past_cache((double)rows * 2 * F * (dh_dtype == SDAMD_F32 ? 4 : 2));
 #define GB_LAUNCH(TD, TH, TO, LD) \
-  (past ? geglu_backward_kernel<TD, TH, TO, true> : geglu_backward_kernel<TD, TH, TO, false>)<<<(nvec + 255) / 256, 256, 0, st>>>( \
-      (const TD*)dout, (const TH*)h, h_scale, (TO*)dh, nvec, VR, F, LD, SP, h_dtype)
+  geglu_backward_launch<TD, TH, TO>(dim3((nvec + 255) / 256), st, past, q != nullptr, (const TD*)dout, (const TH*)h, h_scale, (TO*)dh, nvec, VR, F, \
+                                    LD, SP, h_dtype, (unsigned char*)q, q_scale, q_fmt)
 #define GB_H(TD, TO) \
   { if (h_dtype == SDAMD_F32) GB_LAUNCH(TD, float, TO, 2 * F); else if (h_dtype == SDAMD_BF16) GB_LAUNCH(TD, bf16_t, TO, 2 * F); else GB_LAUNCH(TD, unsigned char, TO, ldq); }
   if (dout_dtype == SDAMD_F32) { if (dh_dtype == SDAMD_F32) GB_H(float, float) else GB_H(float, bf16_t) }

@@ -1057,9 +1057,11 @@ def geglu_train(h, dtype=torch.float8_e4m3fn, out_dtype=None):
     return out, kept
 
 
-def geglu_backward(dout, h, out_dtype=None):
+def geglu_backward(dout, h, out_dtype=None, blocks=None):
     """Gradient of GeGLU with respect to its input, [..., 2F]: (dout gelu(gate) | dout value gelu'(gate)) from dout [..., F]
-    float32 / bfloat16 and h, the input itself or its 8-bit checkpoint (Blocks8, ``geglu_train``).  ``out_dtype`` default: dout's."""
+    float32 / bfloat16 and h, the input itself or its 8-bit checkpoint (Blocks8, ``geglu_train``).  ``out_dtype`` default: dout's.
+    ``blocks`` = float8_e4m3fn / float8_e5m2: returns (gradient, ``quantize8(gradient, blocks)``), the operands of
+    ``linear8_weight_grad`` and of the ``linear8`` that takes the gradient on, for bfloat16 and F % 128 == 0 in the same pass."""
     is8 = isinstance(h, Blocks8)
     if is8 and h.block_rows != 1:
         raise _lib.SdamdError("geglu_backward: h is a weight")
@@ -1071,9 +1073,13 @@ def geglu_backward(dout, h, out_dtype=None):
     Fh = dout.shape[-1]
     rows = dout.numel() // Fh
     _fits("geglu_backward", 2 * Fh)
+    fmt = 0 if blocks is None else _code8(blocks)
     dh = dout.new_empty(h.shape, dtype=out_dtype)
+    d8 = _blocks8_empty(dh, blocks) if fmt and Fh % BLOCK8 == 0 and out_dtype == torch.bfloat16 else None
+    qp, sp = (0, 0) if d8 is None else (d8.q.data_ptr(), d8.scale.data_ptr())
     if rows:
-        _run8(dev, "sdamd_geglu_backward", (dout.data_ptr(), (h.q if is8 else h).data_ptr(), h.scale.data_ptr() if is8 else 0, dh.data_ptr(), rows, Fh, dcode, hcode, ocode),
+        _run8(dev, "sdamd_geglu_backward", (dout.data_ptr(), (h.q if is8 else h).data_ptr(), h.scale.data_ptr() if is8 else 0, dh.data_ptr(),
+                                            qp, sp, rows, Fh, dcode, hcode, ocode, fmt),
               lambda: ("geglu_backward", dh.numel() * (dh.element_size() + (1 if is8 else h.element_size()) + dout.element_size() / 2),
                        f"rows{rows} F{Fh}", 0.0))
-    return dh
+    return dh if not fmt else (dh, quantize8(dh, blocks) if d8 is None else d8)

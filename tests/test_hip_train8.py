@@ -618,6 +618,24 @@ def test_geglu_train_into_blocks(rows, F, dtype, fmt):
         assert ((part - slack).max(1) <= top * s).all() and ((part + slack).max(1) > top * s / 2).all()
 
 
+@pytest.mark.parametrize("rows,F", [(1, 128), (5, 384), (300, 640), (3, 1), (7, 200), (0, 128)])
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+def test_geglu_backward_with_blocks(rows, F, out, fmt):
+    h, dout = rnd(rows + F, (rows, 2 * F), BF16, 1.5).to(DEV), rnd(F, (rows, F), BF16, 0.1).to(DEV)
+    if rows > 2:
+        h[1, 0], h[2, -1] = float("inf"), float("nan")
+    kept = ops.quantize8(h)
+    for given in (h, kept):
+        want = ops.geglu_backward(dout, given, out_dtype=out)
+        dh, d8 = ops.geglu_backward(dout, given, out_dtype=out, blocks=fmt)
+        two = ops.quantize8(want, fmt)
+        assert torch.equal(dh.nan_to_num(7.0), want.nan_to_num(7.0)) and d8.shape == (rows, 2 * F) and d8.dtype == fmt
+        assert torch.equal(d8.q.view(torch.uint8), two.q.view(torch.uint8)) and torch.equal(d8.scale, two.scale)
+    with pytest.raises(TypeError):
+        ops.geglu_backward(dout, h, blocks=BF16)
+
+
 def test_geglu_gradient_against_differences():
     rows, F, step = 3, 50, 1e-5
     h, dout = rnd(1, (rows, 2 * F)), rnd(2, (rows, F))
@@ -656,9 +674,9 @@ def ffn_step(x, w1, b1, w2, b2, gamma, beta, dy, w1t, w2t):
     dyb = dy.to(BF16)
     dw2, db2 = ops.linear8_weight_grad(dyb, g8)
     dg = ops.linear8(dyb, w2t, fmt=E5M2)
-    dh = ops.geglu_backward(dg, h8)
+    dh, dh8 = ops.geglu_backward(dg, h8, blocks=E5M2)
     dw1, db1 = ops.linear8_weight_grad(dh, n8)
-    dn = ops.linear8(dh, w1t, fmt=E5M2)
+    dn = ops.linear8(dh8, w1t)
     dx, dgamma, dbeta = ops.layernorm_backward(dn, x, gamma, mean, rstd, residual=dy)
     return y, dx, dw1, db1, dw2, db2, dgamma, dbeta
 

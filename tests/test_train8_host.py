@@ -38,7 +38,7 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_layernorm_train(P, P, 0, P, P, P, P, 1 << 24, 768, 1e-5, 0, 0, 0), "too many rows")
     refused(L.sdamd_layernorm_backward(P, P, 0, P, P, P, 0, P, P, P, P, 1 << 30, 1 << 29, 8, 0, 0, 0, 0), "too many rows")
     refused(L.sdamd_geglu_train(P, P, 0, P, P, 1 << 40, 64, 0, 0, 2, 0), "too large")
-    refused(L.sdamd_geglu_backward(P, P, 0, P, 1 << 40, 64, 0, 0, 0, 0), "too large")
+    refused(L.sdamd_geglu_backward(P, P, 0, P, 0, 0, 1 << 40, 64, 0, 0, 0, 0, 0), "too large")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 0, 4, 4, 2, 0), "bad shape")
     refused(L.sdamd_linear8_weight_grad(P, P, P, P, P, 0, 0, 4, 4, 4, 1, 0), "unsupported dtype")
     need = L.sdamd_linear8_weight_grad_ws_bytes(65536, 320, 320)
@@ -57,8 +57,10 @@ def test_c_boundary_refuses_bad_arguments():
     refused(L.sdamd_geglu_train(P, P, 0, P, P, 4, 64, 2, 2, 2, 0), "unsupported dtypes")
     refused(L.sdamd_geglu_train(P, P, 0, P, P, 4, 64, 1, 0, 2, 0), "unsupported dtypes")
     refused(L.sdamd_geglu_train(P, P, 0, P, P, 4, 64, 0, 2, 2, 0), "without room")
-    refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 0, 2, 0, 0), "without its scales")
-    refused(L.sdamd_geglu_backward(P, P, 0, P, 4, 64, 2, 0, 0, 0), "unsupported dtypes")
+    refused(L.sdamd_geglu_backward(P, P, 0, P, 0, 0, 4, 64, 0, 2, 0, 0, 0), "without its scales")
+    refused(L.sdamd_geglu_backward(P, P, 0, P, 0, 0, 4, 64, 2, 0, 0, 0, 0), "unsupported dtypes")
+    for args in ((P, 0, 4, 128, 0, 0, 1, 2), (P, P, 4, 128, 0, 0, 0, 2), (P, P, 4, 64, 0, 0, 1, 2), (P, P, 4, 128, 0, 0, 1, 1)):
+        refused(L.sdamd_geglu_backward(P, P, 0, P, *args, 0), "blocks of dh")
 
 
 def test_c_boundary_keeps_launches_below_2_to_32_threads():
