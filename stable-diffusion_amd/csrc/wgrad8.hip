@@ -51,10 +51,12 @@ template <int FMT> __device__ __forceinline__ void w8_to_bf16(u32x4_t v, float s
 }
 __device__ __forceinline__ int w8_swz(int t) { return (t & 3) | (((t >> 3) & 1) << 2); }
 
-// DMA: rows of dy are 16-byte aligned (N % 8 == 0 and an aligned base) and go straight to LDS; otherwise through registers
-// (8192 x 1280 x 1280: 49.7 us; 1284 columns, through registers: 66.8)
-template <int BT_N, int BT_K, int WGN, int WGK, int FMT, bool DMA>
+// How dy gets to LDS.  DMA: its rows are 16-byte aligned (N % 8 == 0 and an aligned base).  ROWS: any other rows of 8 columns or
+// more, through registers (8192 x 1280 x 1280: 50.9 us, 1284 columns: 62).  NARROW: fewer columns, value by value.
+enum W8Rows { W8_DMA, W8_ROWS, W8_NARROW };
+template <int BT_N, int BT_K, int WGN, int WGK, int FMT, W8Rows HOW>
 __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
+  constexpr bool DMA = HOW == W8_DMA;
   constexpr int NT = 64 * WGN * WGK, TN = BT_N / WGN / 16, TK = BT_K / WGK / 16;
   constexpr int ROWN = BT_N * 2, ROWK = BT_K * 2, STAGE = 64 * (ROWN + ROWK);
   constexpr int QI = 64 * BT_K / 16 / NT;                  // 16-byte pieces of x8 per thread and step
@@ -78,22 +80,19 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
   const char* dy0 = reinterpret_cast<const char*>(p.dy) + (size_t)t_begin * p.N * 2;
   const unsigned char* q0 = p.q + (size_t)t_begin * p.KB * B8_BLOCK;
   const unsigned char* s0 = p.qs + (size_t)t_begin * p.SP;
-  unsigned off_d[DI], off_q[QI], off_s[QI];
-  int shift_s[QI];
-#pragma unroll
-  for (int i = 0; i < DI; ++i) {
-    const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-    const int col = n0 + (DMA ? ((c >> 1) ^ w8_swz(t)) * 2 + (c & 1) : c) * 8;          // (DMA: the column whose 16 bytes belong at this place)
-    off_d[i] = (unsigned)t * (unsigned)p.N * 2u + (unsigned)(DMA ? min(col, p.N - 8) : col) * 2u;
-  }
-#pragma unroll
-  for (int i = 0; i < QI; ++i) {
-    const int piece = i * NT + tid, t = piece / (BT_K / 16), kc = min(k0 + piece % (BT_K / 16) * 16, p.KB * B8_BLOCK - 16);
-    off_q[i] = (unsigned)t * (unsigned)(p.KB * B8_BLOCK) + (unsigned)kc;
-    off_s[i] = (unsigned)t * (unsigned)p.SP + (unsigned)(kc / B8_BLOCK & ~3);           // (the word with the scale; a byte load's
-    shift_s[i] = (kc / B8_BLOCK & 3) * 8;                                               //  extension the compiler would wait for at once)
-  }
-  Raw8<bf16_t> rd[DMA ? 1 : DI];
+  // A thread's pieces lie DROWS and QROWS tokens apart, in the same columns.
+  constexpr int DROWS = NT / (ROWN / 16), QROWS = NT / (BT_K / 16);
+  static_assert(NT % (ROWN / 16) == 0 && NT % (BT_K / 16) == 0 && DROWS % 16 == 0, "a piece's place and permutation");
+  const int d_t = tid / (ROWN / 16), d_c = tid % (ROWN / 16), q_t = tid / (BT_K / 16);
+  const int d_col = n0 + (DMA ? ((d_c >> 1) ^ w8_swz(d_t)) * 2 + (d_c & 1) : d_c) * 8;       // (DMA: the column whose 16 bytes belong at this place)
+  const unsigned d_step = (unsigned)DROWS * (unsigned)p.N * 2u;
+  const unsigned off_d = (unsigned)d_t * (unsigned)p.N * 2u + (unsigned)(HOW == W8_NARROW ? 0 : min(d_col, p.N - 8)) * 2u;
+  const int kc = min(k0 + tid % (BT_K / 16) * 16, p.KB * B8_BLOCK - 16);
+  const unsigned q_step = (unsigned)QROWS * (unsigned)(p.KB * B8_BLOCK), s_step = (unsigned)QROWS * (unsigned)p.SP;
+  const unsigned off_q = (unsigned)q_t * (unsigned)(p.KB * B8_BLOCK) + (unsigned)kc;
+  const unsigned off_s = (unsigned)q_t * (unsigned)p.SP + (unsigned)(kc / B8_BLOCK & ~3);    // (the word with the scale; a byte load's
+  const int shift_s = (kc / B8_BLOCK & 3) * 8;                                               //  extension the compiler would wait for at once)
+  u32x4_t rd[DMA ? 1 : DI];
   u32x4_t rq[QI];
   unsigned rs[QI];
   auto request = [&](int s, int buf) {
@@ -101,11 +100,13 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
     const unsigned char* q = q0 + (size_t)s * 64 * p.KB * B8_BLOCK;
     const unsigned char* sc = s0 + (size_t)s * 64 * p.SP;
     const char* d = dy0 + (size_t)s * 64 * p.N * 2;
+    unsigned od = off_d, oq = off_q, os = off_s;
+    asm volatile("" : "+v"(od), "+v"(oq), "+v"(os));       // (or every piece's offset takes a register of its own)
 #pragma unroll
     for (int i = 0; i < QI; ++i) {
-      const bool in = (i * NT + tid) / (BT_K / 16) < left;
-      rq[i] = *reinterpret_cast<const u32x4_t*>(q + (in ? off_q[i] : 0u));
-      rs[i] = *reinterpret_cast<const unsigned*>(sc + (in ? off_s[i] : 0u));
+      const bool in = q_t + i * QROWS < left;
+      rq[i] = *reinterpret_cast<const u32x4_t*>(q + (in ? oq + i * q_step : 0u));
+      rs[i] = *reinterpret_cast<const unsigned*>(sc + (in ? os + i * s_step : 0u));
     }
     auto place = [&](int i) {
       return __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(lds_voidw_t*)(smem + buf * STAGE + (i * NT + (tid & ~63)) * 16));
@@ -114,19 +115,20 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
       if (left >= 64) {
 #pragma unroll
         for (int i = 0; i < DI; ++i)
-          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place(i)), "v"(off_d[i]), "s"(d) : "memory", "m0");
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(place(i)), "v"(od + i * d_step), "s"(d) : "memory", "m0");
       } else {
 #pragma unroll
         for (int i = 0; i < DI; ++i) {
-          const void* src = (i * NT + tid) / (ROWN / 16) < left ? (const void*)(d + off_d[i]) : (const void*)g_wgrad_zero;
+          const void* src = d_t + i * DROWS < left ? (const void*)(d + od + i * d_step) : (const void*)g_wgrad_zero;
           asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(place(i)), "v"(src) : "memory", "m0");
         }
       }
     } else {
 #pragma unroll
       for (int i = 0; i < DI; ++i) {
-        const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-        rd[DMA ? 0 : i] = raw8_load(reinterpret_cast<const bf16_t*>(d) + (size_t)min(t, left - 1) * p.N, n0 + c * 8, p.N);
+        const char* at = d + (d_t + i * DROWS < left ? od + i * d_step : 0u);
+        if constexpr (HOW == W8_ROWS) rd[i] = *reinterpret_cast<const b8_u32x4_a2*>(at);
+        else rd[DMA ? 0 : i] = raw8_load(reinterpret_cast<const bf16_t*>(at), 0, p.N).a;     // (no column past N is looked at)
       }
     }
   };
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
     for (int i = 0; i < QI; ++i) {
       const int piece = i * NT + tid, t = piece / (BT_K / 16), u = piece % (BT_K / 16);
       u32x4_t lo, hi;
-      w8_to_bf16<FMT>(rq[i], b8_scale((int)(rs[i] >> shift_s[i]) & 255), lo, hi);
+      w8_to_bf16<FMT>(rq[i], b8_scale((int)(rs[i] >> shift_s) & 255), lo, hi);
       if (t >= left) { lo = (u32x4_t){0u, 0u, 0u, 0u}; hi = lo; }
       char* d = smem + buf * STAGE + 64 * ROWN + t * ROWK + ((u ^ w8_swz(t)) << 5);
       *reinterpret_cast<u32x4_t*>(d) = lo;
@@ -147,9 +149,9 @@ __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
 #pragma unroll
       for (int i = 0; i < DI; ++i) {
         const int piece = i * NT + tid, t = piece / (ROWN / 16), c = piece % (ROWN / 16);
-        u32x4_t o = rd[DMA ? 0 : i].a;
-        const int s = p.N < 8 ? 0 : max(n0 + c * 8 - (p.N - 8), 0);      // a row's last, partial piece was read s columns early
-        if (s > 0) {
+        u32x4_t o = rd[DMA ? 0 : i];
+        const int s = max(n0 + c * 8 - (p.N - 8), 0);      // a row's last, partial piece was read s columns early
+        if (HOW == W8_ROWS && s > 0) {
           if (s & 4) o = (u32x4_t){o[2], o[3], 0u, 0u};
           if (s & 2) o = (u32x4_t){o[1], o[2], o[3], 0u};
           if (s & 1) o = (u32x4_t){o[0] >> 16 | o[1] << 16, o[1] >> 16 | o[2] << 16, o[2] >> 16 | o[3] << 16, o[3] >> 16};
@@ -284,7 +286,7 @@ static W8Plan w8_plan(int T, int N, int K) {
   const int kp = b8_kblocks(K) * B8_BLOCK, all = (T + 63) / 64;
   W8Plan best{};
   double best_us = 0;
-  for (int big = 0; big < 2; ++big) {
+  for (int big = 0; big < (N < 8 ? 1 : 2); ++big) {
     const int b = big ? 256 : 128, tn = (N + b - 1) / b, tk = (kp + b - 1) / b;
     const long long tiles = (long long)tn * tk;
     for (int want : tries) {
@@ -308,11 +310,11 @@ extern "C" size_t sdamd_linear8_weight_grad_ws_bytes(int T, int N, int K) {
   return w.splits > 1 ? (size_t)w.splits * ((size_t)N * K + N) * sizeof(float) : 0;
 }
 
-template <int B, int WGN, int WGK, int FMT, bool DMA>
+template <int B, int WGN, int WGK, int FMT, W8Rows HOW>
 static int w8_launch(const W8Args& p, int splits, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
   constexpr int lds = 2 * 64 * 2 * B * 2;
-  auto k = wgrad8_kernel<B, B, WGN, WGK, FMT, DMA>;
+  auto k = wgrad8_kernel<B, B, WGN, WGK, FMT, HOW>;
   const hipError_t e = sd_lds_opt_in(done, (const void*)k, lds);
   if (e != hipSuccess) return sdamd_set_error(2, "linear8_weight_grad: %s", hipGetErrorString(e));
   k<<<dim3(p.tiles_n * p.tiles_k, splits), 64 * WGN * WGK, lds, st>>>(p);
@@ -336,8 +338,9 @@ extern "C" int sdamd_linear8_weight_grad(const void* dy, const void* x8, const u
   const bool dma = N % 8 == 0 && ((uintptr_t)dy & 15) == 0;
   int rc;
 #define W8_FMT(F)                                                                                          \
-  rc = w.big ? (dma ? w8_launch<256, 4, 2, F, true>(p, w.splits, st) : w8_launch<256, 4, 2, F, false>(p, w.splits, st)) \
-             : (dma ? w8_launch<128, 2, 2, F, true>(p, w.splits, st) : w8_launch<128, 2, 2, F, false>(p, w.splits, st))
+  rc = w.big ? (dma ? w8_launch<256, 4, 2, F, W8_DMA>(p, w.splits, st) : w8_launch<256, 4, 2, F, W8_ROWS>(p, w.splits, st))              \
+     : dma   ? w8_launch<128, 2, 2, F, W8_DMA>(p, w.splits, st)                                                                          \
+     : N < 8 ? w8_launch<128, 2, 2, F, W8_NARROW>(p, w.splits, st) : w8_launch<128, 2, 2, F, W8_ROWS>(p, w.splits, st)
   if (fmt == SDAMD_E4M3) W8_FMT(SDAMD_E4M3); else W8_FMT(SDAMD_E5M2);
 #undef W8_FMT
   if (rc) return rc;
