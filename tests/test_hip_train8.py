@@ -798,3 +798,48 @@ def test_writes_stay_inside():
             _lib.check(L.sdamd_layernorm_train(x.data_ptr(), y.data_ptr(), 0, g.data_ptr(), g.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows, C,
                                                1e-5, 0, code, st()))
             assert all((t[:256] == 7).all() and (t[-256:] == 7).all() for t in (by, bm, br))
+
+
+# ------------------------------------------------------------------ Linear's activations over their whole range
+def activation_sweep(dtype):
+    """Pre-activations from one end of the type to the other, dense around -52.1 and -88.7, where the exponential in x / (1 +
+    exp(-c x)) leaves float32's range for c = 1.702 and 1, and what f32 arithmetic gives there in 64 bits."""
+    v = np.concatenate([np.arange(-1000, 1000, 0.37), np.arange(-130, -40, 0.01), np.arange(-1, 1, 1e-3),
+                        np.linspace(-1e4, 1e4, 401), np.array([0.0, -0.0, 1e-30, -1e-30, 1e30, -1e30, 3e38, -3e38, np.inf, -np.inf, np.nan])])
+    return torch.from_numpy(v).to(dtype)
+
+
+def activation_ref(v, act):
+    """(value, bound) of x / (1 + exp(-c x)) for an exact x: the exponential 1 ulp, the digits that its argument lost put back in two
+    roundings, 1 + e half a step, the reciprocal 1 ulp, the product half a step: (2 + 2) + 1 + 2 + 1 = 8 U.  c = 1.702 is a
+    rounded constant and c x a rounded product, which the exponential carries on as 2 U |c x|.  A reciprocal below the smallest
+    normal number 2^-126 may come out as zero (only where |x| < 200)."""
+    c = 1.0 if act == ops.ACT_SILU else 1.702
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = v / (1 + np.exp(-c * v))
+        tol = (8 * U + (0 if act == ops.ACT_SILU else 2 * U * np.minimum(np.abs(c * v), 200))) * np.abs(want) + np.minimum(np.abs(v), 200) * 2.0 ** -126
+    return want, tol
+
+
+# (M, N): the rows kernel with 16, 32 and 64 rows a workgroup, the 128 x 128 tile whole and ragged, the 256 x 256 tile (bf16)
+# whole and ragged
+@pytest.mark.parametrize("M,N", [(16, 200), (30, 333), (200, 333), (2048, 1024), (1500, 2050), (4096, 4096), (4100, 3501)])
+@pytest.mark.parametrize("out", [BF16, F32])
+@pytest.mark.parametrize("act", [ops.ACT_SILU, ops.ACT_QUICK_GELU])
+def test_linear8_activation_over_its_range(M, N, out, act):
+    """Rows of zeros: the residual, or the bias, is the pre-activation."""
+    w, x = ops.quantize8_weight(rnd(1, (N, 40)).to(DEV)), torch.zeros(M, 40, device=DEV)
+    x8 = ops.quantize8(x)
+    v = activation_sweep(out)
+    res = v.repeat(-(-M * N // v.numel()))[:M * N].view(M, N).to(DEV)
+    bias = activation_sweep(F32).flip(0)
+    bias = bias.repeat(-(-N // bias.numel()))[torch.randperm(max(N, bias.numel()), generator=gen(N))[:N]].to(DEV)
+    for pre, got in ((res, ops.linear8(x, w, None, res, act, out)), (res, ops.linear8(x8, w, None, res, act, out)),
+                     (bias.expand(M, N), ops.linear8(x8, w, bias, None, act, out))):
+        pre, got = np64(pre), np64(got)
+        want, tol = activation_ref(pre, act)
+        if out == BF16:
+            tol = tol + UB * np.abs(want)
+        fin = np.isfinite(pre)
+        close(got[fin], want[fin], tol[fin], f"act {act}")
+        assert np.array_equal(got[~fin], want[~fin], equal_nan=True)         # inf -> inf, NaN -> NaN, -inf 0 -> NaN
