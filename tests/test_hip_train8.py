@@ -887,3 +887,35 @@ def test_linear8_products_that_cancel(M, N):
             assert (ops.linear8(x8, w8, out_dtype=F32) == 2.0 ** (16 - d)).all()
             got = ops.linear8(x8, w8, out_dtype=BF16)
             assert (got <= 2.0 ** (16 - d)).all() and (got >= (2.0 ** (16 - d) if d <= kept else 0.0)).all(), (at, d)
+
+
+# one width for each form of the kernel (lanes a row, vectors a lane), all but one of them ragged; rows that give a workgroup of the
+# form's RP rows two or three turns, the last of them short
+LNB_FORMS = [(65, 64, 599), (190, 64, 299), (333, 32, 599), (500, 16, 599), (700, 16, 299), (1001, 8, 299), (1500, 8, 299), (2047, 8, 599),
+             (4095, 2, 299), (8191, 1, 299), (12288, 1, 300)]
+
+
+@pytest.mark.parametrize("C,RP,turns", LNB_FORMS)
+@pytest.mark.parametrize("xt,dt,skip", [(F32, F32, True), (BF16, BF16, False), (E4M3, BF16, True), (E5M2, F32, False)])
+def test_layernorm_backward_joins_many_rows(C, RP, turns, xt, dt, skip):
+    """Weight gradients through partial sums: every form of the kernel, workgroups with several turns, x of every type."""
+    rows = RP * turns - RP // 2
+    assert _lib.lib().sdamd_layernorm_backward_ws_bytes(rows, C) == -(-turns // -(-turns // 256)) * 8 * C       # (so many workgroups leave partial sums)
+    x = rnd(C, (rows, C)) + 0.5
+    dy, gamma = rnd(C + 1, (rows, C), dt, 0.1), 1 + 0.2 * rnd(3, (C,))
+    if xt in (E4M3, E5M2):
+        given = ops.quantize8(x.to(DEV), xt)
+        vals, ot = given.dequantize(F32), dt
+    else:
+        given = vals = x.to(xt).to(DEV)
+        ot = xt
+    res = rnd(9, (rows, C), ot) if skip else None
+    _, mean, rstd = ops.layernorm_train(vals, gamma.to(DEV), torch.zeros(C, device=DEV))
+    call = lambda: ops.layernorm_backward(dy.to(DEV), given, gamma.to(DEV), mean, rstd, None if res is None else res.to(DEV))  # noqa: E731
+    dx, dg, db = call()
+    w_dx, w_dg, w_db, tol, e_g, mag_g = backward_ref(np64(dy), np64(vals), np64(gamma), None if res is None else np64(res), 1e-5)
+    close(dx, w_dx, tol + (UB * np.abs(w_dx) if ot == BF16 else 0), "dx")
+    # a column's sum: at most 3 rows after one another, 3 shuffles, 1 + 3 over the waves, 16 partial rows and 16 lanes of them
+    close(dg, w_dg, e_g + 48 * U * mag_g, "dgamma")
+    close(db, w_db, 48 * U * np.abs(np64(dy)).sum(0), "dbeta")
+    assert all(torch.equal(a, b) for a, b in zip(call(), (dx, dg, db)))          # the same bits every run
