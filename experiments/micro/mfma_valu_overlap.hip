@@ -1,6 +1,7 @@
 // Does the vector stream of one wave (or of the other waves of a SIMD) overlap with in-flight MFMAs on gfx950?
 // Per loop iteration: 8 MFMAs and / or 32 vector instructions, interleaved 1 : 4 in program order; cycles per iteration
-// from s_memtime, at 1, 2 and 3 waves per SIMD.   build: hipcc -O3 --offload-arch=gfx950 mfma_valu_overlap.hip -o mvo
+// from s_memtime, at 1, 2 and 3 waves per SIMD.
+// build: hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_valu_overlap.hip -o mvo
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
