@@ -738,9 +738,11 @@ def _code8(dtype):
     return _FMT8[dtype]
 
 
-# the current device's number and a stream's handle without the Python objects around them (2 us a call); results come from
-# new_empty (1.2 us against 1.6 of torch.empty with a device)
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# the current device's number and a stream's handle without the Python objects around them (2 us a call), where this torch has
+# them: the names are its own, and a build without GPU support lacks them; results come from new_empty (1.2 us against 1.6 of
+# torch.empty with a device)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 _entry = {}              # C entry points by name

@@ -1,10 +1,14 @@
 """CPU-only checks of the 8-bit and training operators: arguments are refused before anything is launched, at the C
 boundary and in Python, and the host-side plans hold."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import sd_amd  # noqa: F401
 from sd_amd import _lib, ops
+from conftest import ROOT
 
 L = _lib.lib()
 P = 4096            # an address that is never read: every call below is refused on the host
@@ -111,3 +115,28 @@ def test_workspaces_cover_their_plans():
         need = L.sdamd_layernorm_backward_ws_bytes(rows, c)
         assert need % (8 * c) == 0 and need <= min(rows, 512) * 8 * c and (need > 0) == (rows > 1000)
     assert L.sdamd_layernorm_backward_ws_bytes(4, 12289) == 0
+
+
+def test_import_without_torch_s_private_names():
+    """A torch without GPU support lacks the two shortcuts: the module is imported all the same, and the public calls take their
+    place."""
+    code = """
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import sd_amd
+from sd_amd import _lib, diffusion, ops, pipeline
+assert ops._current_device is torch.cuda.current_device
+class Stream:
+    cuda_stream = 1234
+torch.cuda.current_stream = lambda i: Stream if i == 5 else None
+assert ops._raw_stream(5) == 1234
+try:
+    ops.quantize8(torch.zeros(4, 200))
+except _lib.SdamdError as e:
+    assert "HIP device" in str(e)
+else:
+    raise AssertionError
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
