@@ -250,7 +250,8 @@ int sdamd_attention(const void* q, const void* k, const void* v, void* out, int 
  * KB up to a multiple of 4 (4-byte aligned).  Weights (e4m3) share a byte over 128 rows: scale [ceil(N/128)][SP].
  * A scale is the smallest power of two with max |finite x| <= max(type) * scale (1 for a block of zeros); values are rounded
  * to nearest even.  NaN stays NaN; an infinity becomes NaN in e4m3 and stays in e5m2.
- * fmt: SDAMD_E4M3 | SDAMD_E5M2.  Odd widths and element-aligned pointers are taken everywhere else. */
+ * fmt: SDAMD_E4M3 | SDAMD_E5M2.  Odd widths and element-aligned pointers are taken everywhere else.  Results overlap no
+ * operand and no other result, unless it says so. */
 /* x [rows] of K values, row stride ldx elements */
 int sdamd_quant8(const void* x, void* q, unsigned char* scale, long long rows, int K, long long ldx, int dtype, int fmt,
                  void* stream);
@@ -265,7 +266,7 @@ int sdamd_dequant8(const void* q, const unsigned char* scale, void* out, long lo
  * weight blocks.  out and residual are out_dtype.  BF16: the scaled 8-bit matrix instruction, which cuts the products of 8
  * consecutive k toward zero at 2^-13 of the largest one's power of two and adds the rest in f32 (1e-5 of usual sums; where the
  * largest products cancel, the others keep 13 bits); F32: exact products summed in f32 at a third of the rate.  act: none,
- * quick-gelu, silu.  N, K <= 2^24. */
+ * quick-gelu, silu.  N, K <= 2^24.  out may be residual itself; it is refused if it overlaps an operand otherwise. */
 int sdamd_linear8_quantises(int M, int N, int K, int out_dtype);
 int sdamd_linear8(const void* x, const unsigned char* x_scale, const void* w, const unsigned char* w_scale, void* out,
                   const float* bias, const void* residual, int M, int N, int K, int act, int x_dtype, int fmt,

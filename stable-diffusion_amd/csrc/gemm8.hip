@@ -598,6 +598,11 @@ static int g8_rows_launch(G8Args p, hipStream_t st) {
   return 0;
 }
 
+// do the bytes [a, a + an) and [b, b + bn) meet
+static bool g8_overlap(const void* a, size_t an, const void* b, size_t bn) {
+  return b && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+}
+
 template <int FMT, bool EXACT, typename TO>
 static int g8_launch(const G8Args& p, int x_dtype, hipStream_t st) {
   if (g8_few_rows(p.M, p.N, p.K, EXACT)) {
@@ -630,6 +635,12 @@ extern "C" int sdamd_linear8(const void* x, const unsigned char* x_scale, const 
   SD_CHECK((((uintptr_t)w | (x_dtype >= SDAMD_E4M3 ? (uintptr_t)x : 0)) & 15) == 0 && (((uintptr_t)w_scale | (uintptr_t)x_scale) & 3) == 0,
            "linear8: blocks have to be 16-byte aligned, their scales 4-byte aligned");
   G8Args p{x, x_scale, (const unsigned char*)w, w_scale, out, bias, residual, M, N, K, b8_kblocks(K), b8_scale_stride(K), act, 0, 0};
+  // (a workgroup stores while others still read; of the residual each reads what it stores itself)
+  const size_t blocks = (size_t)p.KB * B8_BLOCK, size = (size_t)M * N * (out_dtype == SDAMD_F32 ? 4 : 2);
+  SD_CHECK(!g8_overlap(out, size, x, x_dtype >= SDAMD_E4M3 ? M * blocks : (size_t)M * K * (x_dtype == SDAMD_F32 ? 4 : 2)) &&
+           !g8_overlap(out, size, x_dtype >= SDAMD_E4M3 ? x_scale : nullptr, (size_t)M * p.SP) && !g8_overlap(out, size, w, N * blocks) &&
+           !g8_overlap(out, size, w_scale, (size_t)b8_kblocks(N) * p.SP) && !g8_overlap(out, size, bias, (size_t)N * 4) &&
+           (out == residual || !g8_overlap(out, size, residual, size)), "linear8: out overlaps an operand");
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (out_dtype == SDAMD_F32) rc = fmt == SDAMD_E4M3 ? g8_launch<SDAMD_E4M3, true, float>(p, x_dtype, st) : g8_launch<SDAMD_E5M2, true, float>(p, x_dtype, st);

@@ -782,6 +782,12 @@ def _dev8(name, first, *others):
     return first.device
 
 
+def _overlap(a, b):
+    """Do two contiguous tensors share memory."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
+
+
 def _fits(name, *sizes):
     """Sizes that cross the C boundary as ints (ctypes would cut them silently)."""
     if max(sizes) > 0x7fffffff:
@@ -899,7 +905,7 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
     scaled 8-bit products, which are cut toward zero at 2^-13 of the power of two of the largest of 8 consecutive ones and then
     added in float32 (1e-5 of usual sums, a hundredth of the result's own rounding; where the largest products cancel, what is
     left of the others has those 13 bits); a float32 result is summed in float32 from exact products at a third of that rate.
-    ``out`` may be the residual, not x."""
+    ``out`` may be the residual itself and overlaps no other operand."""
     is8 = isinstance(x, Blocks8)
     if not (isinstance(w, Blocks8) and w.block_rows == BLOCK8):
         raise _lib.SdamdError("linear8: w has to come from quantize8_weight")
@@ -927,8 +933,8 @@ def linear8(x, w, bias=None, residual=None, act=ACT_NONE, out_dtype=None, fmt=to
         out = xt.new_empty(shape, dtype=out_dtype)
     elif not (out.dtype == out_dtype and out.is_contiguous() and tuple(out.shape) == shape):
         raise _lib.SdamdError("linear8: out %s %s has to be a contiguous %s %s" % (out.dtype, tuple(out.shape), out_dtype, shape))
-    elif M and out.data_ptr() == xt.data_ptr():
-        raise _lib.SdamdError("linear8: out is x, which other columns still read")
+    elif M and (out.data_ptr() == xt.data_ptr() or (xt.is_contiguous() and _overlap(out, xt))):
+        raise _lib.SdamdError("linear8: out overlaps x, which other columns still read")
     xcode = f8 = _code8(x.dtype if is8 else fmt)
     if not is8:
         xcode = _code(x.dtype)

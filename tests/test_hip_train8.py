@@ -919,3 +919,39 @@ def test_layernorm_backward_joins_many_rows(C, RP, turns, xt, dt, skip):
     close(dg, w_dg, e_g + 48 * U * mag_g, "dgamma")
     close(db, w_db, 48 * U * np.abs(np64(dy)).sum(0), "dbeta")
     assert all(torch.equal(a, b) for a, b in zip(call(), (dx, dg, db)))          # the same bits every run
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+@pytest.mark.parametrize("M", [5, 64, 1100])
+def test_linear8_out_beside_its_operands(M, out):
+    """x, bias, residual and out from one buffer: next to one another they are taken, one element into one another refused; out may
+    be the residual."""
+    K, N = 256, 320
+    es = torch.empty(0, dtype=out).element_size()
+    w = ops.quantize8_weight(rnd(1, (N, K)).to(DEV))
+    x, res, bias = rnd(2, (M, K), out).to(DEV), rnd(3, (M, N), out).to(DEV), rnd(4, (N,)).to(DEV)
+    want = ops.linear8(x, w, bias, res, out_dtype=out)
+    buf = torch.empty((M * K + 2 * M * N) * es + N * 4, dtype=torch.uint8, device=DEV)
+    cut = lambda at, n, dtype, shape: buf[at:at + n * torch.empty(0, dtype=dtype).element_size()].view(dtype).view(shape)  # noqa: E731
+    def fill():
+        xs, bs = cut(0, M * K, out, (M, K)), cut((M * K + M * N) * es, N, F32, (N,))
+        rs = cut((M * K + M * N) * es + N * 4, M * N, out, (M, N))
+        return xs.copy_(x), bs.copy_(bias), rs.copy_(res)
+    xs, bs, rs = fill()
+    o = cut(M * K * es, M * N, out, (M, N))
+    assert torch.equal(ops.linear8(xs, w, bs, rs, out_dtype=out, out=o), want)
+    assert torch.equal(ops.linear8(xs, w, bs, rs, out_dtype=out, out=rs), want)
+    xs, bs, rs = fill()
+    keep = buf.clone()
+    for at in (-es, es):                                 # into x's end, into the bias
+        bad = cut(M * K * es + at, M * N, out, (M, N))
+        with pytest.raises(_lib.SdamdError, match="overlaps"):
+            ops.linear8(xs, w, bs, rs, out_dtype=out, out=bad)
+    bad = cut((M * K + M * N) * es + N * 4 - es, M * N, out, (M, N))     # one element before the residual
+    with pytest.raises(_lib.SdamdError, match="overlaps"):
+        ops.linear8(xs, w, None, rs, out_dtype=out, out=bad)
+    x8 = ops.quantize8(xs)
+    row = ops.Blocks8(x8.q[:1], x8.scale[:1], (1, K))
+    with pytest.raises(_lib.SdamdError, match="overlaps"):
+        ops.linear8(row, w, out=x8.q.view(-1)[128:128 + 2 * N].view(BF16).view(1, N))
+    assert torch.equal(buf, keep)                        # nothing was written

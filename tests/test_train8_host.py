@@ -140,3 +140,22 @@ else:
     raise AssertionError
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
+
+
+def test_linear8_out_overlaps_no_operand():
+    """M = 70, N = 40, K = 200 (blocks of 256 bytes, 4 scale bytes), far apart but for the one that is named."""
+    M, N, K = 70, 40, 200
+    base = {"x": 1 << 32, "x_scale": 2 << 32, "w": 3 << 32, "w_scale": 4 << 32, "bias": 6 << 32, "residual": 7 << 32}
+    out = 5 << 32
+    for code, es in ((0, 4), (1, 2)):
+        end = M * N * es
+        size = {"x": M * 256, "x_scale": M * 4, "w": N * 256, "w_scale": 4, "bias": N * 4, "residual": end}
+        for name, n in size.items():
+            step = 16 if name in ("x", "w") else 4
+            for at in (out + end - step, out - n + step) + ((out,) if name != "residual" else (out + step, out - step)):
+                a = dict(base, **{name: at})
+                refused(L.sdamd_linear8(a["x"], a["x_scale"], a["w"], a["w_scale"], out, a["bias"], a["residual"], M, N, K, 0, 2, 2, code, 0), "overlaps")
+    for x_dtype, n in ((0, 4), (1, 2)):                  # rows that the kernel quantises itself
+        refused(L.sdamd_linear8(out - 40 * K * n + n, 0, base["w"], base["w_scale"], out, 0, 0, 40, N, K, 0, x_dtype, 2, 1, 0), "overlaps")
+    t = torch.zeros(100)
+    assert ops._overlap(t[:50], t[49:]) and ops._overlap(t[10:20], t) and not ops._overlap(t[:50], t[50:]) and not ops._overlap(t[50:], t[:50])
