@@ -84,8 +84,8 @@ __device__ __forceinline__ void attn_body(const AttnArgs& p) {
   constexpr bool ONES = D < DV;
   // When the head dim also leaves a spare padded K column (d = 40: DK = 48), the softmax reference rides in the QK^T
   // product: Q is pre-scaled by scale*log2(e) once, K[:, D] = 1 and Q[:, D] = -m (the query's current reference, kept
-  // bf16-exact), so the MFMA returns scale*s - m and exp2 applies to it directly -- no per-score FMA (16 v_pk_fma_f32
-  // of the 131 VALU instructions per 64-key tile in a VALU-issue-bound loop).  The reference still only moves when a
+  // bf16-exact), so the MFMA returns scale*s - m and exp2 applies to it directly -- no per-score FMA (32 v_fma_f32
+  // per 64-key tile in a VALU-issue-bound loop; with packed instructions, which the build keeps off, it was 16 of 131).  The reference still only moves when a
   // row outgrows it by 2^RESCALE_THR; tiles where it moves subtract the difference explicitly (rare path).
   constexpr bool AUG = BF && DK > D && ONES;
   constexpr bool OPT = AUG && !TRACK;
@@ -288,7 +288,7 @@ __device__ __forceinline__ void attn_body(const AttnArgs& p) {
       const f32x2_t sc2 = {sc, sc}, nm2 = {-m_new, -m_new};
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        // v_pk_fma_f32 (measured: scalar v_fma_f32 + -fno-slp-vectorize is 2.5 % slower here)
+        // (written in pairs, compiled to two v_fma_f32: the build keeps packed f32 instructions off)
         const f32x2_t a = (f32x2_t){s[sub][e], s[sub][e + 1]} * sc2 + nm2;
         const float p0 = __builtin_amdgcn_exp2f(a[0]), p1 = __builtin_amdgcn_exp2f(a[1]);
         s[sub][e] = p0;
