@@ -3,7 +3,7 @@
 #include "blocks8.h"
 
 // ---- rows -> blocks.  q [rows][KB*128], scale [rows][SP]; 16 lanes hold a block, a workgroup takes 16 * UN blocks, all of
-// them requested before the first is used.  36864 x 1280 bf16: 24.9 us = 5.7 TB/s with UN = 2 (1: 31.1, 4: 26.3).
+// them requested before the first is used.  36864 x 1280 bf16: 23 - 24.4 us = 5.9 TB/s with UN = 2 (1: 31.1, 4: 26.3).
 template <typename T, int UN>
 __global__ __launch_bounds__(256) void quant8_kernel(const T* __restrict__ x, unsigned char* __restrict__ q,
                                                      unsigned char* __restrict__ scale, unsigned nblk, int KB, int K,
@@ -35,8 +35,9 @@ __global__ __launch_bounds__(256) void quant8_kernel(const T* __restrict__ x, un
 
 // ---- weights -> 128 x 128 blocks.  One workgroup per block; the weight has any strides (w and w.t() alike).  ALONG = 1: its
 // rows are contiguous, 16 lanes take 128 columns of a row and leave their bytes where they belong; 2: its columns are
-// contiguous, the bytes turn in LDS; 0: neither, value by value.  10240 x 1280 bf16: 12.2 us
-// (3.2 TB/s; value by value 53), its transpose 14.2.
+// contiguous, the bytes turn in LDS; 0: neither, value by value.  10240 x 1280 bf16: 11.1 us
+// (3.5 TB/s; value by value 53), its transpose 13.1; f32 12.8 and 14.8 (5.1 and 4.4 TB/s).  All 800 workgroups are on the
+// chip at once, so loads, reduction and stores follow one another with no other block's beside them.
 template <typename T, int ALONG>
 __global__ __launch_bounds__(256) void quant8_weight_kernel(const T* __restrict__ w, unsigned char* __restrict__ q,
                                                             unsigned char* __restrict__ scale, int N, int K, long long sn,
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(256) void quant8_weight_kernel(const T* __restrict_
   if ((int)blockIdx.x == KB - 1 && KB + t < SP) scale[(size_t)blockIdx.y * SP + KB + t] = 127;
 }
 
-// ---- blocks -> the values they stand for
+// ---- blocks -> the values they stand for.  36864 x 1280 to bf16: 22.2 us = 6.4 TB/s, to f32 41.7.
 template <typename TO>
 __global__ __launch_bounds__(256) void dequant8_kernel(const unsigned char* __restrict__ q, const unsigned char* __restrict__ scale,
                                                        TO* __restrict__ out, unsigned nblk, int KB, int K, int SP, int row_shift, int fmt) {
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(256) void dequant8_kernel(const unsigned char* __re
 
 // ---- GeGLU that keeps its input in 8 bits: h [rows][2F] -> out [rows][F] = value * gelu(gate), of h's type or as blocks of
 // another Linear's operand, and h's blocks.
-// 65536 x 1280 bf16: 114 us = 5.9 TB/s; into blocks 112, where a quantiser behind it makes 170.
+// 65536 x 1280 bf16: 102 - 119 us = 5.7 - 6.6 TB/s, by what the caches hold; into blocks 114, where a quantiser behind it makes 154.
 // F % 128 == 0: the 16 lanes that hold a value block hold the gate block of the same columns too, so h is read once.
 enum GegluOut { GEGLU_DENSE, GEGLU_PAST, GEGLU_BLOCKS };    // PAST: past the cache (b8_past_cache)
 template <typename T, GegluOut OUT>
@@ -150,8 +151,8 @@ __global__ __launch_bounds__(256) void geglu_train_kernel(const T* __restrict__ 
   if (fb == (unsigned)FB - 1 && 2 * FB + sub < SP) scale[(size_t)row * SP + 2 * FB + sub] = 127;
 }
 // any F: a value's block and its gate's do not line up.  A workgroup quantises R whole rows, then gates them; it finds them in
-// the caches the second time.  (10000 x 1000 bf16: 22.5 us, as two launches 28.4; 65536 x
-// 960 107 and 138.  R with 32 blocks together; with 64 and 128 10000 x 1000 f32 takes 40.6 and 41.7 instead of 34.4.)
+// the caches the second time.  (10000 x 1000 bf16: 19 - 22.5 us, as two launches 28.4; 65536 x
+// 960 103 - 107 and 138.  R with 32 blocks together; with 64 and 128 10000 x 1000 f32 takes 40.6 and 41.7 instead of 34.4.)
 template <typename T, bool BLOCKS>
 __global__ __launch_bounds__(256) void geglu_rows_kernel(const T* __restrict__ h, void* __restrict__ out, unsigned char* __restrict__ out_scale,
                                                          unsigned char* __restrict__ q, unsigned char* __restrict__ scale, long long rows, int R,
@@ -231,8 +232,8 @@ __device__ __forceinline__ void gelu_slope(float x, float& gelu, float& slope) {
 
 // ---- GeGLU backward: dvalue = dout gelu(gate), dgate = dout value gelu'(gate); h as values (TH) or as 8-bit blocks
 // (TH = unsigned char).  BLOCKS (F % 128 == 0, dh bf16): dh's blocks too, of the values as dh holds them, the operand of the Linear that
-// takes it on.  65536 x 1280 bf16 from e4m3: 128 us = 5.2 TB/s; with blocks 160, where a quantiser behind it
-// makes 219.
+// takes it on.  65536 x 1280 bf16 from e4m3: 120 us = 5.6 TB/s, 133 right behind its forward pass; with blocks 155, where a quantiser behind it
+// makes 212; from bf16 h 150 (5.6 TB/s), all f32 306.
 template <typename TD, typename TH, typename TO, bool PAST, bool BLOCKS>
 __global__ __launch_bounds__(256) void geglu_backward_kernel(const TD* __restrict__ dout, const TH* __restrict__ h,
                                                              const unsigned char* __restrict__ scale, TO* __restrict__ dh,

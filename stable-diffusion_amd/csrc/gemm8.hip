@@ -11,7 +11,7 @@
 // themselves are off by (2^-4 each, 3.7e-2 of a sum) nothing, so a bf16 result takes this form (4.5 PFLOP/s measured from
 // registers).  But where products of a group cancel, what is left of the others has 13 bits below those two, so it is not
 // an f32 sum: for an f32 result (EXACT) the bytes and their scales go to bf16, which holds them exactly (it has f32's range:
-// scale bytes that this library makes stay inside it), and through
+// scale bytes that this library makes stay inside it; below its smallest number, 2^-133, it rounds), and through
 // v_mfma_f32_16x16x32_bf16, whose products and sums are exact to f32 rounding (1.9 PFLOP/s from registers).
 //
 // Which 32 of a block's 128 values a lane supplies does not matter as long as both operands agree, the scales covering
@@ -131,8 +131,9 @@ template <typename TO> __device__ __forceinline__ void g8_store4(const G8Args& p
 // Workgroups are persistent (PLACES per CU) and run their tiles as one sequence of steps: the first step of the next tile
 // is on its way while the last of this one is multiplied, and its multiplication runs while the stores drain.
 //
-// Measured: 8192^3 435 - 500 us (2.2 - 2.5 PFLOP/s, by the board's power), 36864 x 1280 -> 10240 480 - 525, 16384 x 640 ->
-// 5120 61, f32 results 0.8 PFLOP/s.  Bound by power: without requests and stores the same loop makes 2.7 - 2.8 PFLOP/s, and so
+// Measured: 8192^3 435 - 490 us (2.2 - 2.5 PFLOP/s, by the board's power), 36864 x 1280 -> 10240 450 - 475, 16384 x 640 ->
+// 5120 60 - 64, 4096 x 1280 -> 3840 24; f32 results 8192^3 930 - 950 (1.17 PFLOP/s), 36864 x 1280 -> 10240 935, 16384 x 640 ->
+// 5120 122 - 130, 4096 x 1280 -> 3840 43.  Bound by power: without requests and stores the same loop makes 2.7 - 2.8 PFLOP/s, and so
 // does one with half the LDS reads (4 waves of 128 x 128, 512 registers each, which with its requests and stores was 2 - 15%
 // slower than this).  The requests cost 15%, the stores 5% at K = 8192 and 25% at 640.
 __device__ __forceinline__ void dma16(const void* base, unsigned off, void* lds) {
@@ -554,7 +555,7 @@ static bool g8_few_rows(int rows, int N, int K, bool exact) {
 // every 16 columns anew: no second launch and no buffers for the blocks, half the time of an eager call (64 x 320 -> 1280: 8.7
 // us, first quantised 18.5; 154 x 768 -> 640: 9.8 and 17.6).  On the GPU, us, us first quantised, by the blocks that a compute
 // unit's waves quantise one after the other: 1 x 320 -> 1280 (1) 3.5, 4.8; 16 x 1280 -> 1280 (1) 4.8, 5.6; 32 x 1280 -> 1280 (2)
-// 7.0, 6.1; 64 x 768 -> 640 (4) 8.5, 6.1; 256 x 1024 -> 640 (4) 10.7, 6.7; 64 x 1280 -> 640 (8) 13.4, 7.2; 512 x 320 -> 1280 (12)
+// 7.0, 6.1; 64 x 768 -> 640 (4) 8.6, 6.5; 256 x 1024 -> 640 (4) 9.0, 7.0; 64 x 1280 -> 640 (8) 13.4, 7.2; 512 x 320 -> 1280 (12)
 // 22.7, 8.4, and then the eager call loses too (21.9, 17.8).  So up to 4.
 extern "C" int sdamd_linear8_quantises(int M, int N, int K, int out_dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;

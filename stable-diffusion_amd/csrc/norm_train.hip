@@ -1,4 +1,4 @@
-// LayerNorm forward for training (norm_train.h).  65536 x 320 f32 -> bf16: 21.3 us (5.9 TB/s), -> e4m3 blocks 21.6; 77 x 768: 3.5.
+// LayerNorm forward for training (norm_train.h).  65536 x 320 f32 -> bf16: 21.3 us (5.9 TB/s), -> e4m3 blocks 21.7; 77 x 768: 3.8.
 #include "norm_train.h"
 
 // lanes per row and vectors per lane: at most 4 vectors where the row allows it.  (With 5 or 6 and fewer lanes no lane is

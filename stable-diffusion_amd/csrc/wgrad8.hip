@@ -2,7 +2,10 @@
 //   dW[n][k] = sum_t dy[t][n] x8[t][k],   db[n] = sum_t dy[t][n];   dy [T][N] bf16, x8 [T][KB*128] with a scale per row and 128
 // The reduction runs over tokens, along which the scales change, so the 8-bit instruction (one scale per operand row)
 // cannot take x8.  Its bytes go to bf16 on the way into LDS, scaled: bf16 holds every such value exactly, so all products
-// are exact and the sums are f32, whatever the checkpoint's type.  Bound by the bf16 matrix rate for wide layers.
+// are exact and the sums are f32, whatever the checkpoint's type.  Bound by the bf16 matrix rate for wide layers
+// (16384 x 5120 x 640: 0.72 PFLOP/s, 8192^3 1.1); the narrow ones by their splits: 65536 x 320 x 320 in 54 of them 40 us (floor 13),
+// 16384 x 640 x 640 in 10 35 (11), 8192 x 1280 x 1280 in 5 48 (22).  dy is bf16 as the instruction's other operand: an f32 gradient
+// is rounded by whoever has it, or would take three such products.
 //
 // Workgroup tile BT_N x BT_K of dW, token steps of 64, two LDS buffers.  Both operands arrive as rows of one token and are
 // needed as columns of 8 tokens: ds_read_b64_tr_b16 turns 4 x 16 blocks on the way out of LDS.  A row's 32-byte units (16
@@ -52,7 +55,7 @@ template <int FMT> __device__ __forceinline__ void w8_to_bf16(u32x4_t v, float s
 __device__ __forceinline__ int w8_swz(int t) { return (t & 3) | (((t >> 3) & 1) << 2); }
 
 // How dy gets to LDS.  DMA: its rows are 16-byte aligned (N % 8 == 0 and an aligned base).  ROWS: any other rows of 8 columns or
-// more, through registers (8192 x 1280 x 1280: 50.9 us, 1284 columns: 62).  NARROW: fewer columns, value by value.
+// more, through registers (8192 x 1280 x 1280: 48 us, 1284 columns: 56).  NARROW: fewer columns, value by value.
 enum W8Rows { W8_DMA, W8_ROWS, W8_NARROW };
 template <int BT_N, int BT_K, int WGN, int WGK, int FMT, W8Rows HOW>
 __global__ __launch_bounds__(64 * WGN * WGK) void wgrad8_kernel(W8Args p) {
