@@ -955,3 +955,72 @@ def test_linear8_out_beside_its_operands(M, out):
     with pytest.raises(_lib.SdamdError, match="overlaps"):
         ops.linear8(row, w, out=x8.q.view(-1)[128:128 + 2 * N].view(BF16).view(1, N))
     assert torch.equal(buf, keep)                        # nothing was written
+
+
+# ------------------------------------------------------------------ offsets that pass 32 bits
+BIG = 180000, 12288                                      # 2.2e9 elements
+
+
+def big(seed, shape, dtype=BF16):
+    return torch.randn(shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV, dtype=dtype)
+
+
+def same_rows(whole, rows, part):
+    """The last rows of a long result and the result of those rows alone."""
+    if isinstance(whole, ops.Blocks8):
+        n = part.q.shape[0]
+        return torch.equal(whole.q[-n:].view(torch.uint8), part.q.view(torch.uint8)) and torch.equal(whole.scale[-n:], part.scale)
+    return torch.equal(whole[-rows:], part)
+
+
+def test_long_rows_quantised_and_normalised():
+    R, C, n = *BIG, 9
+    x = big(1, (R, C))
+    x8 = ops.quantize8(x)
+    assert same_rows(x8, n, ops.quantize8(x[-n:])) and same_rows(x8.dequantize(), n, ops.quantize8(x[-n:]).dequantize())
+    g, b = 1 + 0.1 * big(2, (C,), F32), big(3, (C,), F32)
+    y, mean, rstd = ops.layernorm_train(x, g, b)
+    ys, ms, rs = ops.layernorm_train(x[-n:], g, b)
+    assert same_rows(y, n, ys) and same_rows(mean, n, ms) and same_rows(rstd, n, rs)
+    assert same_rows(ops.layernorm_train(x, g, b, out_dtype=E4M3)[0], n, ops.layernorm_train(x[-n:], g, b, out_dtype=E4M3)[0])
+    for given, part in ((x, x[-n:]), (x8, ops.quantize8(x[-n:]))):
+        dx = ops.layernorm_backward(y, given, g, mean, rstd, residual=x)[0]
+        assert same_rows(dx, n, ops.layernorm_backward(ys, part, g, ms, rs, residual=x[-n:])[0])
+
+
+@pytest.mark.parametrize("F", [6144, 6143])
+def test_long_rows_geglu(F):
+    n = 9
+    h = big(1, (BIG[0], 2 * F))
+    out, kept = ops.geglu_train(h)
+    po, pk = ops.geglu_train(h[-n:])
+    assert same_rows(out, n, po) and same_rows(kept, n, pk)
+    assert same_rows(ops.geglu_train(h, out_dtype=E4M3)[0], n, ops.geglu_train(h[-n:], out_dtype=E4M3)[0])
+    dh, d8 = ops.geglu_backward(out, kept, blocks=E5M2)
+    pd, p8 = ops.geglu_backward(po, pk, blocks=E5M2)
+    assert same_rows(dh, n, pd) and same_rows(d8, n, p8) and same_rows(ops.geglu_backward(out, h), n, ops.geglu_backward(po, h[-n:]))
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_long_rows_linear(out):
+    """Past 32 bits in the result and the residual, then in the rows; enough rows alone for the same kernel."""
+    R, C, n = *BIG, 20000
+    for K, N in ((100, C), (C, 16)):
+        x8 = ops.quantize8(big(1, (R, K)))
+        part = ops.Blocks8(x8.q[-n:], x8.scale[-n:], (n, K))
+        w, res = ops.quantize8_weight(big(2, (N, K))), big(3, (R, N), out)
+        whole = ops.linear8(x8, w, residual=res, out_dtype=out)
+        assert same_rows(whole, n, ops.linear8(part, w, residual=res[-n:], out_dtype=out))
+        del x8, res, whole
+
+
+@pytest.mark.parametrize("N,K", [(BIG[1], 16), (16, BIG[1]), (BIG[1] - 3, 16)])
+def test_long_weight_grad(N, K):
+    """Whole numbers, so that sums are exact; only the last rows of dy are not zero."""
+    T, n = BIG[0], 100
+    dy, x = torch.zeros((T, N), dtype=BF16, device=DEV), torch.zeros((T, K), dtype=BF16, device=DEV)
+    dy[-n:], x[-n:] = big(1, (n, N)).round(), big(2, (n, K)).round()
+    x[:1000] = 3
+    dw, db = ops.linear8_weight_grad(dy, ops.quantize8(x))
+    w, b = ops.linear8_weight_grad(dy[-n:].contiguous(), ops.quantize8(x[-n:]))
+    assert torch.equal(dw, w) and torch.equal(db, b) and bool(dw.any())
